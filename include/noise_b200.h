@@ -294,6 +294,89 @@ int noise_fitness_static_max_members(void);
 int noise_fitness_static(const float* losses, int members, int pairs, int mode, float* weights, int32_t* ranks,
                          void* stream);
 
+/* Element types of the operators below. */
+#define NOISE_FP32 0
+#define NOISE_BF16 1
+#define NOISE_FP16 2
+
+/* Norms of the queries and keys for each head together with the position rotation, one launch for both
+ * (utils/model.py:55-58, 86-88, for any number of heads, head widths and layouts). q [B, T, H, D] and
+ * k [B, T, Hk, D] of `dtype`, D contiguous, element strides of the other dimensions {batch, token, head}
+ * in *_stride; pointers 16-byte aligned, strides multiples of 16 bytes. D a multiple of 16, at most 256.
+ * rope: [table][D] fp32 cos | sin, 16-byte aligned; a token's row is positions[b * positions_stride + t],
+ * or t when positions is null. A position outside the table gives NaN rows. wq, wk: optional [D] fp32
+ * weights of the norms. order NOISE_ROTATE_NORM: norm(R x); NOISE_NORM_ROTATE: R norm(x), with
+ * R (x1, x2) = (x1 cos + x2 sin, x2 cos - x1 sin) on the halves and norm(u) = w u / sqrt(mean u^2 + eps).
+ * Forward (backward = 0): q_out, k_out receive the result; they may be q and k themselves.
+ * Backward: dq, dk are the results' gradients, q_out and k_out receive those of q and k, dwq and dwk (given
+ * exactly when wq and wk are) the weights'; a call with weights needs
+ * noise_qk_norm_workspace_bytes(D) of workspace. Its sums over rows run in a fixed order. */
+#define NOISE_ROTATE_NORM 0
+#define NOISE_NORM_ROTATE 1
+typedef struct NoiseQkNorm {
+  int dtype, order, B, T, H, Hk, D;
+  float eps;
+  const float* rope;
+  int64_t table;
+  const int32_t* positions;
+  int64_t positions_stride;
+  const float *wq, *wk;
+  const void *q, *k, *dq, *dk;
+  void *q_out, *k_out;
+  int64_t q_stride[3], k_stride[3], dq_stride[3], dk_stride[3], q_out_stride[3], k_out_stride[3];
+  float *dwq, *dwk;
+} NoiseQkNorm;
+int64_t noise_qk_norm_workspace_bytes(int D);
+int noise_qk_norm_rope(const NoiseQkNorm* args, int backward, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Causal attention with a sliding window and `sinks` first tokens that stay visible, for any length,
+ * grouped heads and padded batches (the fixed model's window attention, utils/model.py:17-31, is sinks = 0).
+ * q [B, Tq, H, D], k and v [B, Tk, Hk, D] (H a multiple of Hk) of bf16 or fp16, D contiguous and a
+ * multiple of 8, at most 128; element strides {batch, token, head}, pointers 16-byte aligned and strides
+ * multiples of 16 bytes. Query row i of a sequence is at position p = offset + i (offset + Tq <= Tk) and
+ * sees key j iff j <= p, and p - j <= window or j < sinks. lengths [B] (optional, on the device): tokens of
+ * sequence b at positions >= lengths[b] are padding: their keys and values are never used, whatever they
+ * hold, and their query rows give zeros (lse -inf).
+ * out [B, Tq, H, D] contiguous, 16-byte aligned; lse [B, H, Tq] fp32, the natural logarithm of each row's
+ * sum of exp(scale q.k) over its visible keys. */
+typedef struct NoiseWindow {
+  int dtype, B, Tq, Tk, H, Hk, D, offset, window, sinks;
+  float scale;
+  const int32_t* lengths;
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  void* out;
+  float* lse;
+} NoiseWindow;
+int noise_window_attention(const NoiseWindow* args, int* status, void* stream);
+
+/* One new token per sequence over a cache: q [B, H, D] (q_stride {batch, -, head}), k and v [B, Tk, Hk, D] as
+ * above, lengths [B] required: the query of sequence b is at position lengths[b] - 1 and its own key and
+ * value are in the cache. lengths[b] = 0 gives zeros. Tq and offset are not read. out [B, H, D]
+ * contiguous; lse [B, H] fp32, optional. */
+int noise_window_token(const NoiseWindow* args, void* stream);
+
+/* Distillation from a teacher's top logits. logits [N, V] (row stride ld) of `dtype`, ids [N, K] int32 or
+ * int64 (row stride ids_ld), teacher [N, K] logits of teacher_dtype (row stride teacher_ld), K <= 1024.
+ * s = softcap tanh(z / softcap) / temperature (softcap 0: z / temperature), p = softmax of a row's teacher
+ * logits / temperature, loss = temperature^2 sum_k p_k (log p_k - s[id_k] + logsumexp(s)). Entries whose id is
+ * outside [0, V) are absent; equal ids add up; a row without an entry above -inf has loss and gradient 0.
+ * lse_in null: loss [N] (and lse [N], optional: logsumexp(s)) are written, and, with grad, the gradient of
+ * sum_n dloss[n] loss[n] (dloss null: of sum_n loss[n]) in the same pass, for
+ * V <= noise_distill_max_vocab(dtype, softcap > 0). lse_in given (the lse of an earlier call): only grad.
+ * grad [N, V] of `dtype`, row stride grad_ld; it must not overlap logits. */
+typedef struct NoiseDistill {
+  int dtype, teacher_dtype, ids_int64, V, K;
+  float temperature, softcap;
+  int64_t N, ld, ids_ld, teacher_ld, grad_ld;
+  const void *logits, *ids, *teacher;
+  const float *dloss, *lse_in;
+  float *loss, *lse;
+  void* grad;
+} NoiseDistill;
+int64_t noise_distill_max_vocab(int dtype, int softcap);
+int noise_distill(const NoiseDistill* args, void* stream);
+
 /* Instrumentation, no reference counterpart: total kernel launches made by this library so far;
  * optional per-kind device timing with CUDA events recorded on the launching stream (kinds: 0 embed,
  * 1 qkv, 2 attention, 3 proj, 4 fc, 5 mlp, 6 head, 7 loss, 8 fitness, 9 update, 10 pack, 11 other).

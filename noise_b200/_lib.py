@@ -76,6 +76,12 @@ SIGNATURES: dict[str, tuple] = {
                                      c_void_p]),
     'noise_fitness_static_max_members': (c_int, []),
     'noise_fitness_static': (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    'noise_qk_norm_workspace_bytes': (c_int64, [c_int]),
+    'noise_qk_norm_rope': (c_int, [c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    'noise_window_attention': (c_int, [c_void_p, c_void_p, c_void_p]),
+    'noise_window_token': (c_int, [c_void_p, c_void_p]),
+    'noise_distill_max_vocab': (c_int64, [c_int, c_int]),
+    'noise_distill': (c_int, [c_void_p, c_void_p]),
     'noise_launch_count': (c_int64, []),
     'noise_profile_enable': (c_int, [c_int]),
     'noise_profile_read': (c_int, [c_void_p, c_void_p, c_int]),
@@ -115,6 +121,35 @@ class NoiseCapture(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ('blocks', 'x0', 'inv0', 'y', 'mid', 'hidden', 'final_x', 'logits',
                                          'token_loss')]
 
+
+Strides3 = c_int64 * 3  # element strides {batch, token, head}
+
+
+class NoiseQkNorm(ctypes.Structure):
+    """struct NoiseQkNorm of include/noise_b200.h."""
+    _fields_ = [(n, c_int) for n in ('dtype', 'order', 'B', 'T', 'H', 'Hk', 'D')] + [
+        ('eps', c_float), ('rope', c_void_p), ('table', c_int64), ('positions', c_void_p), ('positions_stride', c_int64)] + [
+        (n, c_void_p) for n in ('wq', 'wk', 'q', 'k', 'dq', 'dk', 'q_out', 'k_out')] + [
+        (n, Strides3) for n in ('q_stride', 'k_stride', 'dq_stride', 'dk_stride', 'q_out_stride', 'k_out_stride')] + [
+        ('dwq', c_void_p), ('dwk', c_void_p)]
+
+
+class NoiseWindow(ctypes.Structure):
+    """struct NoiseWindow of include/noise_b200.h."""
+    _fields_ = [(n, c_int) for n in ('dtype', 'B', 'Tq', 'Tk', 'H', 'Hk', 'D', 'offset', 'window', 'sinks')] + [
+        ('scale', c_float)] + [(n, c_void_p) for n in ('lengths', 'q', 'k', 'v')] + [
+        (n, Strides3) for n in ('q_stride', 'k_stride', 'v_stride')] + [('out', c_void_p), ('lse', c_void_p)]
+
+
+class NoiseDistill(ctypes.Structure):
+    """struct NoiseDistill of include/noise_b200.h."""
+    _fields_ = [(n, c_int) for n in ('dtype', 'teacher_dtype', 'ids_int64', 'V', 'K')] + [
+        ('temperature', c_float), ('softcap', c_float)] + [
+        (n, c_int64) for n in ('N', 'ld', 'ids_ld', 'teacher_ld', 'grad_ld')] + [
+        (n, c_void_p) for n in ('logits', 'ids', 'teacher', 'dloss', 'lse_in', 'loss', 'lse', 'grad')]
+
+
+byref = ctypes.byref
 
 _lib = None
 

@@ -110,6 +110,15 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
 __device__ __forceinline__ void tma_load_2d_hint(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
                                                  uint64_t policy) {
   asm volatile(
@@ -239,6 +248,12 @@ __device__ __forceinline__ uint64_t smem_desc_sw128_mn(const void* tile) {
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;
   return d;
+}
+
+// The same for MN spans of several 64-element blocks, block_bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(const void* tile, uint32_t block_bytes) {
+  uint64_t d = smem_desc_sw128_mn(tile) & ~((uint64_t)0x3FFF << 16);
+  return d | (uint64_t)(block_bytes >> 4) << 16;
 }
 
 // Instruction descriptor: fp32 accumulator, A/B of the given format (0 = f16, 1 = bf16; 2 = tf32

@@ -1,0 +1,91 @@
+"""Distillation from a teacher's top logits (noise_distill): the loss of each row and its gradient.
+
+With s = softcap tanh(z / softcap) / temperature (softcap 0: z / temperature), p the softmax of a row's teacher
+logits / temperature over its entries and lse = logsumexp(s):
+  loss = temperature^2 sum_k p_k (log p_k - s[id_k] + lse)
+The fixed model's head has softcap 15 (utils/model.py:204). No call is recorded by autograd; calls run on the
+current stream of their tensors' device and keep nothing between calls.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .attention import DTYPE_CODES, check_cuda, launch
+
+MAX_ENTRIES = 1024
+
+
+def _matrix(t: torch.Tensor) -> torch.Tensor:
+    """Rows the kernel can address: columns contiguous, rows not overlapping."""
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) \
+        else t.clone(memory_format=torch.contiguous_format)
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _call(name, logits, ids, teacher, temperature, softcap, dloss=None, lse=None, want_loss=True, want_grad=False):
+    if logits.dim() != 2 or ids.dim() != 2 or teacher.shape != ids.shape or len(ids) != len(logits):
+        raise ValueError(f'{name}: logits [N, V], ids and teacher [N, K] expected, got {tuple(logits.shape)}, '
+                         f'{tuple(ids.shape)} and {tuple(teacher.shape)}')
+    if logits.dtype not in DTYPE_CODES or teacher.dtype not in DTYPE_CODES:
+        raise ValueError(f'{name}: logits and teacher must be fp32, bf16 or fp16, got {logits.dtype} and {teacher.dtype}')
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f'{name}: ids must be int32 or int64, got {ids.dtype}')
+    N, V = logits.shape
+    if not 1 <= ids.shape[1] <= MAX_ENTRIES or V < 1 or V > 1 << 30:
+        raise ValueError(f'{name}: 1 to {MAX_ENTRIES} entries a row and 1 to 2^30 logits, got {ids.shape[1]} and {V}')
+    if not 0 < temperature < float('inf') or not 0 <= softcap < float('inf'):
+        raise ValueError(f'{name}: temperature must be positive and softcap not negative, got {temperature} and {softcap}')
+    for t, what in ((dloss, 'dloss'), (lse, 'lse')):
+        if t is not None and (t.shape != (N,) or t.dtype != torch.float32):
+            raise ValueError(f'{name}: {what} must be fp32 [{N}], got {t.dtype} {tuple(t.shape)}')
+    if want_loss and want_grad:
+        limit = int(_lib.load().noise_distill_max_vocab(DTYPE_CODES[logits.dtype], int(softcap > 0)))
+        if V > limit:
+            raise ValueError(f'{name}: loss and gradient in one pass take at most {limit} logits a row of {logits.dtype}, '
+                             f'got {V}; use distill_loss and distill_backward')
+    dev = check_cuda(name, logits, ids, teacher, dloss, lse)
+    loss = torch.empty(N, dtype=torch.float32, device=dev) if want_loss else None
+    out_lse = torch.empty(N, dtype=torch.float32, device=dev) if want_loss else None
+    grad = torch.empty(N, V, dtype=logits.dtype, device=dev) if want_grad else None
+    if N:
+        logits, ids, teacher = _matrix(logits), _matrix(ids), _matrix(teacher)
+        dloss = None if dloss is None else dloss.contiguous()
+        lse = None if lse is None else lse.contiguous()
+        a = _lib.NoiseDistill()
+        a.dtype, a.teacher_dtype, a.ids_int64 = DTYPE_CODES[logits.dtype], DTYPE_CODES[teacher.dtype], ids.dtype == torch.int64
+        a.N, a.V, a.K, a.temperature, a.softcap = N, V, ids.shape[1], temperature, softcap
+        a.ld, a.ids_ld, a.teacher_ld, a.grad_ld = _ld(logits), _ld(ids), _ld(teacher), V
+        a.logits, a.ids, a.teacher = logits.data_ptr(), ids.data_ptr(), teacher.data_ptr()
+        for field, t in (('dloss', dloss), ('lse_in', lse), ('loss', loss), ('lse', out_lse), ('grad', grad)):
+            if t is not None:
+                setattr(a, field, t.data_ptr())
+        launch('noise_distill', dev, _lib.byref(a))
+    return loss, out_lse, grad
+
+
+def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, *, temperature: float = 1.0,
+                 softcap: float = 0.0):
+    """Losses of logits [N, V] against the teacher's entries: ids [N, K] (int32 or int64, K up to 1,024) and their
+    logits teacher [N, K]. An id outside [0, V) marks an absent entry, equal ids add up, and a row without an entry
+    above -inf has loss 0. Returns (loss fp32 [N], lse fp32 [N]); lse is what distill_backward needs."""
+    return _call('distill_loss', logits, ids, teacher, temperature, softcap)[:2]
+
+
+def distill_backward(dloss: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
+                     lse: torch.Tensor, *, temperature: float = 1.0, softcap: float = 0.0) -> torch.Tensor:
+    """Gradient [N, V] of sum_n dloss[n] loss[n] with respect to the logits, from distill_loss's inputs and lse."""
+    if dloss is None or lse is None:
+        raise ValueError('distill_backward: dloss and lse are required')
+    return _call('distill_backward', logits, ids, teacher, temperature, softcap, dloss, lse, False, True)[2]
+
+
+def distill_loss_grad(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, *, temperature: float = 1.0,
+                      softcap: float = 0.0, dloss: torch.Tensor | None = None):
+    """Losses and the gradient of sum_n dloss[n] loss[n] (dloss None: of their sum) in one pass that reads the logits
+    once. Returns (loss fp32 [N], grad [N, V] of the logits' type)."""
+    loss, _, grad = _call('distill_loss_grad', logits, ids, teacher, temperature, softcap, dloss, None, True, True)
+    return loss, grad
