@@ -350,6 +350,15 @@ typedef struct NoiseWindow {
 } NoiseWindow;
 int noise_window_attention(const NoiseWindow* args, int* status, void* stream);
 
+/* Gradient of noise_window_attention, bf16 only: args as given to it, with the out and lse it wrote. dout
+ * [B, Tq, H, D] (element strides dout_stride {batch, token, head}, 16-byte aligned rows) is out's gradient; dq, dk, dv
+ * receive those of q, k, v, contiguous and 16-byte aligned. Padding rows get zeros, and what q, k, v and dout
+ * hold there is not used. Every sum runs in a fixed order. The workspace (16-byte aligned) depends on the shape only. */
+int64_t noise_window_backward_workspace_bytes(const NoiseWindow* args);
+int noise_window_attention_backward(const NoiseWindow* args, const void* dout, const int64_t* dout_stride, void* dq,
+                                    void* dk, void* dv, void* workspace, size_t workspace_bytes, int* status,
+                                    void* stream);
+
 /* One new token per sequence over a cache: q [B, H, D] (q_stride {batch, -, head}), k and v [B, Tk, Hk, D] as
  * above, lengths [B] required: the query of sequence b is at position lengths[b] - 1 and its own key and
  * value are in the cache. lengths[b] = 0 gives zeros. Tq and offset are not read. out [B, H, D]

@@ -6,6 +6,7 @@ library is missing or cannot be loaded, every call raises; nothing falls back to
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / 'libnoise_b200.so'
@@ -17,8 +18,8 @@ STATUS_NAMES = {
     6: 'larger than the static scratch array holds',
 }
 
-c_void_p, c_int, c_float, c_int64, c_uint32, c_size_t, c_uint64 = (
-    ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64, ctypes.c_uint32, ctypes.c_size_t,
+c_char_p, c_void_p, c_int, c_float, c_int64, c_uint32, c_size_t, c_uint64 = (
+    ctypes.c_char_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64, ctypes.c_uint32, ctypes.c_size_t,
     ctypes.c_uint64)
 
 # name -> (restype, argtypes); the single source of truth for what the Python side binds.
@@ -59,7 +60,7 @@ SIGNATURES: dict[str, tuple] = {
                                    c_float, c_float, c_void_p]),
     'noise_fitness_workspace_bytes': (c_size_t, [c_int]),
     'noise_fitness': (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
-    'noise_update_sum_fe_adamw': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_uint32,
+    'noise_update_sum_fe_adamw': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_char_p, c_void_p, c_int, c_float, c_uint32,
                                           c_uint32, c_void_p, c_float, c_float, c_float, c_float, c_float, c_int,
                                           c_void_p, c_void_p]),
     'noise_adamw_region': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float,
@@ -77,11 +78,14 @@ SIGNATURES: dict[str, tuple] = {
     'noise_fitness_static_max_members': (c_int, []),
     'noise_fitness_static': (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     'noise_qk_norm_workspace_bytes': (c_int64, [c_int]),
-    'noise_qk_norm_rope': (c_int, [c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
-    'noise_window_attention': (c_int, [c_void_p, c_void_p, c_void_p]),
-    'noise_window_token': (c_int, [c_void_p, c_void_p]),
+    'noise_qk_norm_rope': (c_int, [c_char_p, c_int, c_void_p, c_size_t, c_void_p]),
+    'noise_window_attention': (c_int, [c_char_p, c_void_p, c_void_p]),
+    'noise_window_backward_workspace_bytes': (c_int64, [c_char_p]),
+    'noise_window_attention_backward': (c_int, [c_char_p, c_void_p, c_char_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                c_size_t, c_void_p, c_void_p]),
+    'noise_window_token': (c_int, [c_char_p, c_void_p]),
     'noise_distill_max_vocab': (c_int64, [c_int, c_int]),
-    'noise_distill': (c_int, [c_void_p, c_void_p]),
+    'noise_distill': (c_int, [c_char_p, c_void_p]),
     'noise_launch_count': (c_int64, []),
     'noise_profile_enable': (c_int, [c_int]),
     'noise_profile_read': (c_int, [c_void_p, c_void_p, c_int]),
@@ -122,34 +126,12 @@ class NoiseCapture(ctypes.Structure):
                                          'token_loss')]
 
 
-Strides3 = c_int64 * 3  # element strides {batch, token, head}
-
-
-class NoiseQkNorm(ctypes.Structure):
-    """struct NoiseQkNorm of include/noise_b200.h."""
-    _fields_ = [(n, c_int) for n in ('dtype', 'order', 'B', 'T', 'H', 'Hk', 'D')] + [
-        ('eps', c_float), ('rope', c_void_p), ('table', c_int64), ('positions', c_void_p), ('positions_stride', c_int64)] + [
-        (n, c_void_p) for n in ('wq', 'wk', 'q', 'k', 'dq', 'dk', 'q_out', 'k_out')] + [
-        (n, Strides3) for n in ('q_stride', 'k_stride', 'dq_stride', 'dk_stride', 'q_out_stride', 'k_out_stride')] + [
-        ('dwq', c_void_p), ('dwk', c_void_p)]
-
-
-class NoiseWindow(ctypes.Structure):
-    """struct NoiseWindow of include/noise_b200.h."""
-    _fields_ = [(n, c_int) for n in ('dtype', 'B', 'Tq', 'Tk', 'H', 'Hk', 'D', 'offset', 'window', 'sinks')] + [
-        ('scale', c_float)] + [(n, c_void_p) for n in ('lengths', 'q', 'k', 'v')] + [
-        (n, Strides3) for n in ('q_stride', 'k_stride', 'v_stride')] + [('out', c_void_p), ('lse', c_void_p)]
-
-
-class NoiseDistill(ctypes.Structure):
-    """struct NoiseDistill of include/noise_b200.h."""
-    _fields_ = [(n, c_int) for n in ('dtype', 'teacher_dtype', 'ids_int64', 'V', 'K')] + [
-        ('temperature', c_float), ('softcap', c_float)] + [
-        (n, c_int64) for n in ('N', 'ld', 'ids_ld', 'teacher_ld', 'grad_ld')] + [
-        (n, c_void_p) for n in ('logits', 'ids', 'teacher', 'dloss', 'lse_in', 'loss', 'lse', 'grad')]
-
-
-byref = ctypes.byref
+# Argument blocks of the model operators, packed in one step (filling a ctypes structure of thirty fields costs
+# more than a small launch); each follows its struct in include/noise_b200.h field by field.
+QK_NORM = struct.Struct('7if QqQq 8Q 18q 2Q')
+WINDOW = struct.Struct('10if 4Q 9q 2Q')
+STEPS = struct.Struct('3q')  # element strides {batch, token, head}
+DISTILL = struct.Struct('5i2f 5q 3Q 2Q 2Q Q')
 
 _lib = None
 

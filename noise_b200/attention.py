@@ -21,65 +21,81 @@ ORDERS = {'rotate_norm': 0, 'norm_rotate': 1}
 NORM_EPS = torch.finfo(torch.float32).eps
 
 
-def check_cuda(name: str, *tensors) -> torch.device:
+def device_index(name: str, *tensors) -> int:
     """The one CUDA device of the tensors (None entries are skipped)."""
-    dev = tensors[0].device
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and (t.device != dev or t.device.type != 'cuda'):
-            raise ValueError(f'{name}: every tensor must be on one CUDA device, got {t.device} and {dev}')
-    return dev
+        if t is not None and (t.get_device() != index or index < 0):
+            raise ValueError(f'{name}: every tensor must be on one CUDA device, got {t.device} and {tensors[0].device}')
+    return index
 
 
-def launch(name: str, dev: torch.device, *args) -> None:
-    """One library call on dev's current stream (the last argument of every entry point)."""
-    if dev.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+def launch(name: str, device: int, *args) -> None:
+    """One library call on the device's current stream (the last argument of every entry point)."""
+    if device == torch.cuda.current_device():
+        # the raw handle of torch.cuda.current_stream(device), without building a Stream object
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
     else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+        with torch.cuda.device(device):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
 
 
-def _addressable(t: torch.Tensor, broadcast: bool = False) -> bool:
-    """16-byte rows that the kernels can step through: D contiguous, aligned pointer and strides."""
-    unit = 16 // t.element_size()
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
-        return False
-    if t.data_ptr() % 16:
-        return False
-    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
-        if n > 1 and (s % unit or s < 0 or (s == 0 and not broadcast)):
-            return False
-    return True
+def _pointer(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _rows(t: torch.Tensor, broadcast: bool = False) -> torch.Tensor:
-    return t if _addressable(t, broadcast) else t.clone(memory_format=torch.contiguous_format)
+def _steps(t: torch.Tensor, broadcast: bool):
+    """Element strides {batch, token, head} if the kernels can step through t, else None: D contiguous, 16-byte
+    aligned rows, no dimension broadcast (unless allowed). A dimension of one element is never stepped along."""
+    sb, st, sh, sd = t.stride()
+    B, T, H, D = t.shape
+    if B == 1:
+        sb = 0
+    if T == 1:
+        st = 0
+    if H == 1:
+        sh = 0
+    if (sd != 1 and D != 1) or t.data_ptr() & 15 or (sb | st | sh) * t.element_size() & 15:
+        return None
+    if not broadcast and ((B > 1 and not sb) or (T > 1 and not st) or (H > 1 and not sh)):
+        return None
+    return sb, st, sh
 
 
-def _strides(t: torch.Tensor):
-    """Element strides {batch, token, head}; a dimension of one element is never stepped along."""
-    return _lib.Strides3(*(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])))
+def _rows(t: torch.Tensor, broadcast: bool = False):
+    """t, or a contiguous copy where its layout cannot be addressed, and its steps."""
+    steps = _steps(t, broadcast)
+    if steps is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        steps = _steps(t, broadcast)
+    return t, steps
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 # ------------------------------------------------------------------------------------------------
 # norms of queries and keys with the rotation
 # ------------------------------------------------------------------------------------------------
-def _qk_args(q, k, rope, positions, q_weight, k_weight, order, eps) -> _lib.NoiseQkNorm:
+def _qk_check(q, k, rope, positions, q_weight, k_weight, order):
+    """Refuses what noise_qk_norm_rope does not take; (B, T, H, Hk, D, positions' batch stride)."""
     name = 'qk_norm_rope'
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
         raise ValueError(f'{name}: q [B, T, H, D] and k [B, T, Hk, D] expected, got {tuple(q.shape)} and {tuple(k.shape)}')
     if q.dtype not in DTYPE_CODES or k.dtype != q.dtype:
         raise ValueError(f'{name}: q and k must share fp32, bf16 or fp16, got {q.dtype} and {k.dtype}')
     B, T, H, D = q.shape
-    if D % 16 or not 16 <= D <= 256 or not H or not k.shape[2]:
+    Hk = k.shape[2]
+    if D % 16 or not 16 <= D <= 256 or not H or not Hk:
         raise ValueError(f'{name}: D must be a multiple of 16 up to 256 and heads at least 1, got {tuple(q.shape)}')
     if order not in ORDERS:
         raise ValueError(f'{name}: order must be one of {sorted(ORDERS)}, got {order!r}')
     if rope.dim() != 2 or rope.shape[1] != D or not len(rope) or rope.dtype != torch.float32 or not rope.is_contiguous() \
-            or rope.data_ptr() % 16:
+            or rope.data_ptr() & 15:
         raise ValueError(f'{name}: rope must be a contiguous fp32 [positions, {D}] table of cos | sin, got '
                          f'{rope.dtype} {tuple(rope.shape)}')
-    a = _lib.NoiseQkNorm()
+    stride = 0
     if positions is None:
         if T > len(rope):
             raise ValueError(f'{name}: {T} tokens but a table of {len(rope)} positions')
@@ -88,17 +104,15 @@ def _qk_args(q, k, rope, positions, q_weight, k_weight, order, eps) -> _lib.Nois
                 (T > 1 and positions.stride(-1) != 1):
             raise ValueError(f'{name}: positions must be int32 [T] or [B, T] with contiguous rows, got {positions.dtype} '
                              f'{tuple(positions.shape)}')
-        a.positions = positions.data_ptr()
-        a.positions_stride = positions.stride(0) if positions.dim() == 2 and B > 1 else 0
-    for w, field in ((q_weight, 'wq'), (k_weight, 'wk')):
-        if w is not None:
-            if w.dtype != torch.float32 or w.shape != (D,) or not w.is_contiguous():
-                raise ValueError(f'{name}: weights must be contiguous fp32 [{D}], got {w.dtype} {tuple(w.shape)}')
-            setattr(a, field, w.data_ptr())
-    a.dtype, a.order, a.B, a.T, a.H, a.Hk, a.D = DTYPE_CODES[q.dtype], ORDERS[order], B, T, H, k.shape[2], D
-    a.eps = eps
-    a.rope, a.table = rope.data_ptr(), len(rope)
-    return a
+        if positions.dim() == 2 and B > 1:
+            stride = positions.stride(0)
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype != torch.float32 or w.shape != (D,) or not w.is_contiguous()):
+            raise ValueError(f'{name}: weights must be contiguous fp32 [{D}], got {w.dtype} {tuple(w.shape)}')
+    return B, T, H, Hk, D, stride
+
+
+_NO_STEPS = (0, 0, 0)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, *, positions: torch.Tensor | None = None,
@@ -111,20 +125,23 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, *, positi
     t row t), and a position outside the table gives NaN rows. q_weight, k_weight: fp32 [D] weights of the
     norms. out: (q_out, k_out) to write to, of any addressable layout (a cache's rows, or q and k themselves).
     Returns (q_out, k_out)."""
-    a = _qk_args(q, k, rope, positions, q_weight, k_weight, order, eps)
+    B, T, H, Hk, D, stride = _qk_check(q, k, rope, positions, q_weight, k_weight, order)
     if out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        q_out, k_out = _like(q), _like(k)
+        q_step, k_step = (T * H * D, H * D, D), (T * Hk * D, Hk * D, D)
     else:
         q_out, k_out = out
-        for o, x in ((q_out, q), (k_out, k)):
-            if o.shape != x.shape or o.dtype != x.dtype or not _addressable(o):
-                raise ValueError('qk_norm_rope: out must have the shapes and type of q and k, 16-byte aligned rows')
-    dev = check_cuda('qk_norm_rope', q, k, rope, positions, q_weight, k_weight, q_out, k_out)
-    q, k = _rows(q, True), _rows(k, True)
-    a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
-    a.q_stride, a.k_stride, a.q_out_stride, a.k_out_stride = _strides(q), _strides(k), _strides(q_out), _strides(k_out)
-    launch('noise_qk_norm_rope', dev, _lib.byref(a), 0, None, 0)
+        q_step, k_step = _steps(q_out, False), _steps(k_out, False)
+        if q_out.shape != q.shape or k_out.shape != k.shape or q_out.dtype != q.dtype or k_out.dtype != q.dtype or \
+                q_step is None or k_step is None:
+            raise ValueError('qk_norm_rope: out must have the shapes and type of q and k, 16-byte aligned rows')
+    device = device_index('qk_norm_rope', q, k, rope, positions, q_weight, k_weight, q_out, k_out)
+    (q, qs), (k, ks) = _rows(q, True), _rows(k, True)
+    a = _lib.QK_NORM.pack(DTYPE_CODES[q.dtype], ORDERS[order], B, T, H, Hk, D, eps, rope.data_ptr(), len(rope),
+                          _pointer(positions), stride, _pointer(q_weight), _pointer(k_weight), q.data_ptr(), k.data_ptr(),
+                          0, 0, q_out.data_ptr(), k_out.data_ptr(), *qs, *ks, *_NO_STEPS, *_NO_STEPS, *q_step, *k_step,
+                          0, 0)
+    launch('noise_qk_norm_rope', device, a, 0, None, 0)
     return q_out, k_out
 
 
@@ -134,24 +151,22 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     """Gradients of qk_norm_rope: dq, dk are those of its results, q, k and the rest its inputs. Returns the
     gradients of (q, k, q_weight, k_weight); a weight that was not given has None. The weights' sums run in a
     fixed order."""
-    a = _qk_args(q, k, rope, positions, q_weight, k_weight, order, eps)
-    for g, x in ((dq, q), (dk, k)):
-        if g.shape != x.shape or g.dtype != x.dtype:
-            raise ValueError('qk_norm_rope_backward: dq and dk must have the shapes and type of q and k')
-    dev = check_cuda('qk_norm_rope_backward', q, k, dq, dk, rope, positions, q_weight, k_weight)
-    q, k, dq, dk = _rows(q, True), _rows(k, True), _rows(dq, True), _rows(dk, True)
-    gq, gk = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
+    B, T, H, Hk, D, stride = _qk_check(q, k, rope, positions, q_weight, k_weight, order)
+    if dq.shape != q.shape or dk.shape != k.shape or dq.dtype != q.dtype or dk.dtype != q.dtype:
+        raise ValueError('qk_norm_rope_backward: dq and dk must have the shapes and type of q and k')
+    device = device_index('qk_norm_rope_backward', q, k, dq, dk, rope, positions, q_weight, k_weight)
+    (q, qs), (k, ks), (dq, dqs), (dk, dks) = _rows(q, True), _rows(k, True), _rows(dq, True), _rows(dk, True)
+    gq, gk = _like(q), _like(k)
     gwq, gwk = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
-    a.q, a.k, a.dq, a.dk = q.data_ptr(), k.data_ptr(), dq.data_ptr(), dk.data_ptr()
-    a.q_out, a.k_out = gq.data_ptr(), gk.data_ptr()
-    a.q_stride, a.k_stride, a.dq_stride, a.dk_stride = _strides(q), _strides(k), _strides(dq), _strides(dk)
-    a.q_out_stride, a.k_out_stride = _strides(gq), _strides(gk)
     ws, need = None, 0
     if gwq is not None or gwk is not None:
-        need = int(_lib.load().noise_qk_norm_workspace_bytes(q.shape[3]))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        a.dwq, a.dwk = (None if g is None else g.data_ptr() for g in (gwq, gwk))
-    launch('noise_qk_norm_rope', dev, _lib.byref(a), 1, None if ws is None else ws.data_ptr(), need)
+        need = int(_lib.load().noise_qk_norm_workspace_bytes(D))
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    a = _lib.QK_NORM.pack(DTYPE_CODES[q.dtype], ORDERS[order], B, T, H, Hk, D, eps, rope.data_ptr(), len(rope),
+                          _pointer(positions), stride, _pointer(q_weight), _pointer(k_weight), q.data_ptr(), k.data_ptr(),
+                          dq.data_ptr(), dk.data_ptr(), gq.data_ptr(), gk.data_ptr(), *qs, *ks, *dqs, *dks,
+                          T * H * D, H * D, D, T * Hk * D, Hk * D, D, _pointer(gwq), _pointer(gwk))
+    launch('noise_qk_norm_rope', device, a, 1, _pointer(ws), need)
     return gq, gk, gwq, gwk
 
 
@@ -167,13 +182,13 @@ class _Status:
             raise ValueError(f'{name}: status must be an int32 word')
         self.name, self.word, self.own = name, status, status is None
 
-    def pointer(self, dev) -> int:
+    def pointer(self, device: int) -> int:
         if self.own:
             if torch.cuda.is_current_stream_capturing():
                 raise ValueError(f'{self.name}: a captured call needs the caller\'s status word')
-            self.word = torch.zeros(1, dtype=torch.int32, device=dev)
-        elif self.word.device != dev:
-            raise ValueError(f'{self.name}: status is on {self.word.device}, the tensors on {dev}')
+            self.word = torch.zeros(1, dtype=torch.int32, device=device)
+        elif self.word.get_device() != device:
+            raise ValueError(f'{self.name}: status is on {self.word.device}, the tensors on cuda:{device}')
         return self.word.data_ptr()
 
     def finish(self):
@@ -183,9 +198,10 @@ class _Status:
                 raise _lib.NoiseError(f'{self.name}: device status {_lib.STATUS_NAMES.get(code, code)}')
 
 
-def _window_args(name, q, k, v, window, sinks, lengths, scale, token) -> _lib.NoiseWindow:
-    dims = 3 if token else 4
-    if q.dim() != dims or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[-1] != k.shape[-1]:
+def _window_check(name, q, k, v, window, sinks, lengths, offset, scale, token):
+    """Refuses what the kernels do not take; the leading fields of NoiseWindow up to `scale`."""
+    if q.dim() != (3 if token else 4) or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or \
+            q.shape[-1] != k.shape[3]:
         raise ValueError(f'{name}: q {"[B, H, D]" if token else "[B, Tq, H, D]"} and k, v [B, Tk, Hk, D] expected, got '
                          f'{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}')
     if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -200,27 +216,21 @@ def _window_args(name, q, k, v, window, sinks, lengths, scale, token) -> _lib.No
         raise ValueError(f'{name}: {Tq} queries need 1 to 2^30 keys, at least as many, got {Tk}')
     if B > 65535 or H > 65535:
         raise ValueError(f'{name}: at most 65,535 sequences and heads a call')
-    window = Tk if window is None else int(window)
+    window = Tk if window is None else min(int(window), Tk)
+    sinks = min(int(sinks), Tk)
     if window < 0 or sinks < 0:
         raise ValueError(f'{name}: window and sinks cannot be negative, got {window} and {sinks}')
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0 < scale < float('inf'):
         raise ValueError(f'{name}: scale must be positive, got {scale}')
-    a = _lib.NoiseWindow()
-    if lengths is not None:
-        if lengths.dtype != torch.int32 or lengths.shape != (B,) or (B > 1 and lengths.stride(0) != 1):
-            raise ValueError(f'{name}: lengths must be contiguous int32 [{B}], got {lengths.dtype} {tuple(lengths.shape)}')
-        a.lengths = lengths.data_ptr()
-    a.dtype, a.B, a.Tq, a.Tk, a.H, a.Hk, a.D = DTYPE_CODES[q.dtype], B, Tq, Tk, H, Hk, D
-    a.offset, a.window, a.sinks, a.scale = Tk - Tq, min(window, Tk), min(int(sinks), Tk), scale
-    return a
-
-
-def _offset(name, a, offset):
-    if offset is not None:
-        if not 0 <= offset <= a.Tk - a.Tq:
-            raise ValueError(f'{name}: offset must lie in [0, {a.Tk - a.Tq}], got {offset}')
-        a.offset = int(offset)
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (B,) or
+                                (B > 1 and lengths.stride(0) != 1)):
+        raise ValueError(f'{name}: lengths must be contiguous int32 [{B}], got {lengths.dtype} {tuple(lengths.shape)}')
+    if offset is None:
+        offset = Tk - Tq
+    elif not 0 <= offset <= Tk - Tq:
+        raise ValueError(f'{name}: offset must lie in [0, {Tk - Tq}], got {offset}')
+    return DTYPE_CODES[q.dtype], B, Tq, Tk, H, Hk, D, int(offset), window, sinks, scale
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int | None, sinks: int = 0, *,
@@ -235,20 +245,52 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     status: an int32 word that a device wait which ran out sets; without one the call waits for the
     GPU and checks its own. Returns (out [B, Tq, H, D], lse fp32 [B, H, Tq])."""
     name = 'window_attention'
-    a = _window_args(name, q, k, v, window, sinks, lengths, scale, False)
-    _offset(name, a, offset)
+    head = _window_check(name, q, k, v, window, sinks, lengths, offset, scale, False)
     st = _Status(name, status)
-    dev = check_cuda(name, q, k, v, lengths)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(a.B, a.H, a.Tq, dtype=torch.float32, device=dev)
+    device = device_index(name, q, k, v, lengths)
+    out = _like(q)
+    lse = torch.empty((head[1], head[4], head[2]), dtype=torch.float32, device=q.device)
     if not out.numel():
         return out, lse
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    a.q, a.k, a.v, a.out, a.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr()
-    a.q_stride, a.k_stride, a.v_stride = _strides(q), _strides(k), _strides(v)
-    launch('noise_window_attention', dev, _lib.byref(a), st.pointer(dev))
+    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
+    a = _lib.WINDOW.pack(*head, _pointer(lengths), q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs,
+                         out.data_ptr(), lse.data_ptr())
+    launch('noise_window_attention', device, a, st.pointer(device))
     st.finish()
     return out, lse
+
+
+def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                              lse: torch.Tensor, window: int | None, sinks: int = 0, *,
+                              lengths: torch.Tensor | None = None, offset: int | None = None,
+                              scale: float | None = None, status: torch.Tensor | None = None):
+    """Gradients of window_attention (bf16): dout is out's, and out, lse are what it returned for the same
+    arguments. Padding rows get zeros. Sums run in a fixed order. Returns (dq, dk, dv)."""
+    name = 'window_attention_backward'
+    head = _window_check(name, q, k, v, window, sinks, lengths, offset, scale, False)
+    if q.dtype != torch.bfloat16:
+        raise ValueError(f'{name}: bf16 only, got {q.dtype}')
+    if dout.shape != q.shape or out.shape != q.shape or dout.dtype != q.dtype or out.dtype != q.dtype:
+        raise ValueError(f'{name}: dout and out must have the shape and type of q')
+    if lse.shape != (head[1], head[4], head[2]) or lse.dtype != torch.float32:
+        raise ValueError(f'{name}: lse must be fp32 [B, H, Tq], got {lse.dtype} {tuple(lse.shape)}')
+    st = _Status(name, status)
+    device = device_index(name, q, k, v, dout, out, lse, lengths)
+    if not q.numel():
+        return torch.empty_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    dq, dk, dv = _like(q), _like(k), _like(v)
+    (q, qs), (k, ks), (v, vs), (dout, gs) = _rows(q), _rows(k), _rows(v), _rows(dout)
+    out, lse = out.contiguous(), lse.contiguous()
+    if out.data_ptr() & 15:
+        out = out.clone()
+    a = _lib.WINDOW.pack(*head, _pointer(lengths), q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs,
+                         out.data_ptr(), lse.data_ptr())
+    need = _lib.load().noise_window_backward_workspace_bytes(a)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    launch('noise_window_attention_backward', device, a, dout.data_ptr(), _lib.STEPS.pack(*gs), dq.data_ptr(),
+           dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), need, st.pointer(device))
+    st.finish()
+    return dq, dk, dv
 
 
 def window_attention_token(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor,
@@ -259,16 +301,14 @@ def window_attention_token(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, le
     name = 'window_attention_token'
     if lengths is None:
         raise ValueError(f'{name}: lengths are required')
-    a = _window_args(name, q, k, v, window, sinks, lengths, scale, True)
-    dev = check_cuda(name, q, k, v, lengths)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    head = _window_check(name, q, k, v, window, sinks, lengths, None, scale, True)
+    device = device_index(name, q, k, v, lengths)
+    out = _like(q)
     if not out.numel():
         return out
-    if not _addressable(q):
-        q = q.clone(memory_format=torch.contiguous_format)
-    k, v = _rows(k), _rows(v)
-    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    a.q_stride = _lib.Strides3(q.stride(0) if a.B > 1 else 0, 0, q.stride(1) if a.H > 1 else 0)
-    a.k_stride, a.v_stride = _strides(k), _strides(v)
-    launch('noise_window_token', dev, _lib.byref(a))
+    q4, qs = _rows(q.unsqueeze(1))
+    (k, ks), (v, vs) = _rows(k), _rows(v)
+    a = _lib.WINDOW.pack(*head, lengths.data_ptr(), q4.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs,
+                         out.data_ptr(), 0)
+    launch('noise_window_token', device, a)
     return out

@@ -11,19 +11,17 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .attention import DTYPE_CODES, check_cuda, launch
+from .attention import DTYPE_CODES, _pointer, device_index, launch
 
 MAX_ENTRIES = 1024
 
 
-def _matrix(t: torch.Tensor) -> torch.Tensor:
-    """Rows the kernel can address: columns contiguous, rows not overlapping."""
-    return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) \
-        else t.clone(memory_format=torch.contiguous_format)
-
-
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _matrix(t: torch.Tensor):
+    """A matrix whose columns are contiguous and whose rows do not overlap (t, or a copy), and its row stride."""
+    rows, cols = t.shape
+    if (t.stride(1) != 1 and cols != 1) or (t.stride(0) < cols and rows != 1):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride(0) if rows > 1 else cols
 
 
 def _call(name, logits, ids, teacher, temperature, softcap, dloss=None, lse=None, want_loss=True, want_grad=False):
@@ -47,23 +45,20 @@ def _call(name, logits, ids, teacher, temperature, softcap, dloss=None, lse=None
         if V > limit:
             raise ValueError(f'{name}: loss and gradient in one pass take at most {limit} logits a row of {logits.dtype}, '
                              f'got {V}; use distill_loss and distill_backward')
-    dev = check_cuda(name, logits, ids, teacher, dloss, lse)
-    loss = torch.empty(N, dtype=torch.float32, device=dev) if want_loss else None
-    out_lse = torch.empty(N, dtype=torch.float32, device=dev) if want_loss else None
-    grad = torch.empty(N, V, dtype=logits.dtype, device=dev) if want_grad else None
+    device = device_index(name, logits, ids, teacher, dloss, lse)
+    where = logits.device
+    loss = torch.empty(N, dtype=torch.float32, device=where) if want_loss else None
+    out_lse = torch.empty(N, dtype=torch.float32, device=where) if want_loss and not want_grad else None
+    grad = torch.empty(N, V, dtype=logits.dtype, device=where) if want_grad else None
     if N:
-        logits, ids, teacher = _matrix(logits), _matrix(ids), _matrix(teacher)
+        (logits, ld), (ids, ids_ld), (teacher, teacher_ld) = _matrix(logits), _matrix(ids), _matrix(teacher)
         dloss = None if dloss is None else dloss.contiguous()
         lse = None if lse is None else lse.contiguous()
-        a = _lib.NoiseDistill()
-        a.dtype, a.teacher_dtype, a.ids_int64 = DTYPE_CODES[logits.dtype], DTYPE_CODES[teacher.dtype], ids.dtype == torch.int64
-        a.N, a.V, a.K, a.temperature, a.softcap = N, V, ids.shape[1], temperature, softcap
-        a.ld, a.ids_ld, a.teacher_ld, a.grad_ld = _ld(logits), _ld(ids), _ld(teacher), V
-        a.logits, a.ids, a.teacher = logits.data_ptr(), ids.data_ptr(), teacher.data_ptr()
-        for field, t in (('dloss', dloss), ('lse_in', lse), ('loss', loss), ('lse', out_lse), ('grad', grad)):
-            if t is not None:
-                setattr(a, field, t.data_ptr())
-        launch('noise_distill', dev, _lib.byref(a))
+        a = _lib.DISTILL.pack(DTYPE_CODES[logits.dtype], DTYPE_CODES[teacher.dtype], ids.dtype == torch.int64, V,
+                              ids.shape[1], temperature, softcap, N, ld, ids_ld, teacher_ld, V, logits.data_ptr(),
+                              ids.data_ptr(), teacher.data_ptr(), _pointer(dloss), _pointer(lse), _pointer(loss),
+                              _pointer(out_lse), _pointer(grad))
+        launch('noise_distill', device, a)
     return loss, out_lse, grad
 
 

@@ -6,7 +6,12 @@ Z = scale max sum_d |q_d k_d| over the pairs, every probability has a relative e
 delta = 2 (D 2^-24 Z + 2^-24 (2 Z + 8)) + 2^-21. P is then rounded to the input type, u = eps / 2 each, and the
 products add in fp32. With A = sum p |v|: |out - want| <= (u + delta) A + u |want| + (keys) 2^-24 A, taken with
 keys 2^-24 inside delta. fp16 holds P below 2^-14 with an absolute half step of 2^-25: keys 2^-25 max|v| more.
-lse: delta + 2^-22 |lse|."""
+lse: delta + 2^-22 |lse|.
+
+Gradients: P and dS are rounded to bf16 once each. dS = P (dP - Delta), where Delta comes from the rounded
+output, itself off by (u + delta) A + u |out|; with size = P (|dO| |V|^T + |dO| . sum p |v|), |dS| <= size and its error is
+at most (3 u + 2 delta) size. Then |dV - want| <= (u + delta) P^T |dO| + u |want|, |dQ - want| <= (3 u + 2 delta) size |K| + u |want|,
+and the same for dK."""
 import pytest
 import torch
 
@@ -89,6 +94,89 @@ def test_forward(case):
     status = torch.zeros(1, dtype=torch.int32, device='cuda')
     again, lse2 = window_attention(qc, kc, vc, window, sinks, status=status, **kw)
     assert torch.equal(out, again) and torch.equal(lse, lse2) and status.item() == 0
+
+
+def check_backward(got, do, q, k, v, window, sinks, lengths, offset):
+    want = oo.window_attention_backward(do, q, k, v, window, sinks, lengths, offset)
+    d, u = deltas(q, k), 2.0 ** -8
+    for name, g, w, mag, part in zip(('dq', 'dk', 'dv'), got, want[:3], want[3:], (3 * u + 2 * d, 3 * u + 2 * d, u + d)):
+        err = (g.double().cpu() - w).abs()
+        tol = part * mag + u * w.abs()
+        assert (err <= tol).all(), (name, (err - tol).max().item(), err.max().item())
+        # a wrong sum would also show as a bias: the errors' norm stays near the roundings' (well below their bound)
+        if w.norm() > 0:
+            assert err.norm() <= 2 * u * w.norm() + 0.5 * (part * mag).norm(), (name, err.norm() / w.norm())
+
+
+@pytest.mark.parametrize('case', [c for c in CASES if c[8] == 'bf16'] + [
+    (1, 1000, 1000, 8, 1, 64, 30, 5, 'bf16', None, None),      # split: shared heads, few key tiles, sinks
+    (1, 2100, 2100, 2, 2, 64, 40, 3, 'bf16', None, None),      # split sinks, even tiles whole
+    (2, 900, 900, 6, 1, 128, 800, 0, 'bf16', (900, 333), None),
+    (2, 1100, 1300, 4, 1, 96, 64, 140, 'bf16', (1300, 900), None),
+])
+def test_backward(case):
+    from noise_b200.attention import window_attention, window_attention_backward
+    q, k, v, do, qc, kc, vc, dc, window, sinks, lengths, offset, kw = build(case)
+    out, lse = window_attention(qc, kc, vc, window, sinks, **kw)
+    got = window_attention_backward(dc, qc, kc, vc, out, lse, window, sinks, **kw)
+    check_backward(got, do, q, k, v, window, sinks, lengths, offset)
+    status = torch.zeros(1, dtype=torch.int32, device='cuda')
+    again = window_attention_backward(dc, qc, kc, vc, out, lse, window, sinks, status=status, **kw)
+    assert status.item() == 0
+    for a, b in zip(got, again):
+        assert torch.equal(a, b)
+
+
+def test_oracle_gradient_matches_differences():
+    """The float64 formulas that the kernel is held to, against central differences of the float64 forward."""
+    g = torch.Generator().manual_seed(31)
+    q, k, v, do = (torch.randn(1, 9, n, 8, generator=g, dtype=torch.float64) for n in (2, 1, 1, 2))
+    lengths = (8,)
+    grads = oo.window_attention_backward(do, q, k, v, 3, 1, lengths)[:3]
+    for x, gx in zip((q, k, v), grads):
+        for at in range(0, x.numel(), 5):
+            old = x.view(-1)[at].item()
+            vals = []
+            for h in (1e-5, -1e-5):
+                x.view(-1)[at] = old + h
+                vals.append((oo.window_attention(q, k, v, 3, 1, lengths)[0] * do).sum().item())
+            x.view(-1)[at] = old
+            assert abs((vals[0] - vals[1]) / 2e-5 - gx.reshape(-1)[at].item()) < 1e-8
+
+
+def test_backward_layouts_graph_and_stream():
+    """Strided operands and gradients; a captured forward and backward that follows its inputs; another stream."""
+    from noise_b200.attention import window_attention, window_attention_backward
+    g = torch.Generator().manual_seed(19)
+    qkv = randn(g, 2, 310, 8, 64, dtype=torch.bfloat16).cuda()
+    q, k, v = qkv[:, :, :4], qkv[:, :, 4:6], qkv[:, :, 6:]
+    do = randn(g, 2, 4, 310, 64, dtype=torch.bfloat16).cuda().transpose(1, 2)
+    lengths = torch.tensor([310, 211], dtype=torch.int32, device='cuda')
+    status = torch.zeros(1, dtype=torch.int32, device='cuda')
+    kw = dict(lengths=lengths, status=status)
+
+    def both(q, k, v, do):
+        out, lse = window_attention(q, k, v, 100, 4, **kw)
+        return (out, lse, *window_attention_backward(do, q, k, v, out, lse, 100, 4, **kw))
+
+    want = both(q, k, v, do)
+    for a, b in zip(want, both(*(t.contiguous() for t in (q, k, v, do)))):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = both(q, k, v, do)
+    qkv.copy_(randn(g, *qkv.shape, dtype=torch.bfloat16))
+    lengths.copy_(torch.tensor([40, 309]))
+    graph.replay()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = both(q, k, v, do)
+    torch.cuda.synchronize()
+    assert status.item() == 0
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
 
 
 def test_layouts():
@@ -210,10 +298,11 @@ def test_token_graph_follows_lengths():
 
 
 def test_empty_batches():
-    from noise_b200.attention import window_attention, window_attention_token
+    from noise_b200.attention import window_attention, window_attention_backward, window_attention_token
     z = torch.zeros(0, 5, 2, 64, dtype=torch.bfloat16, device='cuda')
     assert window_attention(z, z, z, 3)[0].shape == z.shape
     assert window_attention_token(z[:, 0], z, z, torch.zeros(0, dtype=torch.int32, device='cuda'), 3).shape == (0, 2, 64)
     k = torch.zeros(2, 5, 2, 64, dtype=torch.bfloat16, device='cuda')
+    assert window_attention_backward(z, z, z, z, z, torch.zeros(0, 2, 5, device='cuda'), 3)[0].shape == z.shape
     out, lse = window_attention(k[:, :0], k, k, 3)
     assert out.shape == (2, 0, 2, 64) and lse.shape == (2, 2, 0)
