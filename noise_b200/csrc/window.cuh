@@ -34,6 +34,15 @@ __device__ __forceinline__ bool window_all(int qlo, int qhi, int klo, int khi, i
   return khi <= qlo && (qhi - klo <= window || khi < sinks);
 }
 
+// 32 columns of this warp's tensor memory lanes; the wait names the registers, so that no use moves before it.
+__device__ __forceinline__ void tmem_read32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  tmem_ld32_async(taddr, r);
+  tmem_wait_ld_regs(r);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 int make_tmap_bthd(CUtensorMap* map, const void* ptr, int dtype, int B, int T, int heads, int D, const int64_t* stride,
                    uint32_t box_rows);
 int device_sm_count();

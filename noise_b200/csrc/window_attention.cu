@@ -3,10 +3,12 @@
 //
 //   S = scale Q K^T where visible, -inf elsewhere,   O = softmax(S) V,   lse = log sum exp S
 //
-// One pass over the keys: each query row keeps its running maximum m and the sum l of exp(S - m), and its
-// O (in tensor memory) is multiplied by exp(m_old - m_new) when m grows. m is only raised when the tile's
-// maximum exceeds it by more than 8 in the base-2 exponent: P then stays below 2^8, far inside bf16 and
-// fp16, l and O stay fp32, and the rescaling, a read and write of the whole O tile, almost never runs.
+// One pass over the keys: each query row keeps a reference m and the sum l of exp(S - m). m is the maximum of
+// the first tile the row sees, and is raised only when a later tile's P sums to more than 2^10 under it; then
+// the tile is taken again under its new maximum and O (in tensor memory) and l are scaled by exp(m_old - m_new).
+// The sum that l needs anyway thus guards the range, and the usual tile spends no instruction on a maximum:
+// 153 -> FWD us at B 8, T 2048, 8 heads of 64, window 1024, 4 sinks. P, l and O only meet as P / l and O / l, so
+// a reference below the maximum costs no accuracy.
 //
 // One CTA = two consecutive tiles of 128 queries of one head; they share every key and value tile the CTA
 // streams, while one tile's products overlap the other's exponentials. Key tiles: the sinks' first, then
@@ -42,6 +44,11 @@ struct WinFwd {
   static constexpr uint32_t kTmemCols = DP == 64 ? 256 : 512;
   static constexpr int kCtas = DP == 64 ? 2 : 1;
 };
+
+// Sum of a tile's P above which the tile is taken again under a higher maximum. A tile under its own maximum sums
+// to at most 128, so anything above says that the maximum has grown; up to 2^10 P stays exact enough in bf16 and
+// fp16 (below 65,504) and the fp32 sums far from overflow.
+constexpr float kWinTileSum = 1024.f;
 
 // The key tiles of a CTA: sink tiles [0, sink), then tiles lo .. hi.
 struct KeyWalk {
@@ -239,6 +246,7 @@ __global__ void __launch_bounds__(WinFwd<DP>::kThreads, WinFwd<DP>::kCtas)
     const uint32_t tS = tmem + L::kGroupCols * g + lanes, tO = tS + KT;
     if (g < active) {
       const float c = p.scale * 1.4426950408889634f;
+      const float2 c2 = make_float2(c, c);
       const int q = p.offset + i;
       const int qlo = q_first(g) + quarter * 32, qhi = qlo + 31;  // this warp's positions
       float m = -INFINITY;
@@ -253,76 +261,73 @@ __global__ void __launch_bounds__(WinFwd<DP>::kThreads, WinFwd<DP>::kCtas)
           break;
         }
         tc_fence_after();
-        float sv[KT];
-#pragma unroll
-        for (int h = 0; h < KT / 64; ++h) {
-          uint32_t a[32], bb[32];
-          tmem_ld32_async(tS + 64 * h, a);
-          tmem_ld32_async(tS + 64 * h + 32, bb);
-          tmem_wait_ld_regs(a);
-          tmem_wait_ld_regs(bb);
-#pragma unroll
-          for (int u = 0; u < 32; ++u) sv[64 * h + u] = __uint_as_float(a[u]), sv[64 * h + 32 + u] = __uint_as_float(bb[u]);
-        }
-        float top = -INFINITY;
-        uint32_t none = 0;
-#pragma unroll
-        for (int h = 0; h < KT / 32; ++h) {
-          const int kc = kt * KT + 32 * h;
-          if (window_none(qlo, qhi, kc, kc + 31, p.window, p.sinks)) {
-            none |= 1u << h;
-          } else {
-            if (!window_all(qlo, qhi, kc, kc + 31, p.window, p.sinks)) {
+        const int k0 = kt * KT;
+        // P of the tile, with m as it stands; `raise` (for the whole warp) first lifts m to the rows' maxima
+        bool raise = !__all_sync(0xffffffffu, m > -INFINITY);
+        uint32_t w[KT / 2];
+        float2 t2[2];
+        while (true) {
+          if (raise) {
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int h = 0; h < KT / 32; ++h) {
+              const int kc = k0 + 32 * h;
+              if (window_none(qlo, qhi, kc, kc + 31, p.window, p.sinks)) continue;
+              float sv[32];
+              tmem_read32(tS + 32 * h, sv);
 #pragma unroll
               for (int u = 0; u < 32; ++u)
-                if (!window_sees(q, kc + u, p.window, p.sinks)) sv[32 * h + u] = -INFINITY;
+                if (window_sees(q, kc + u, p.window, p.sinks)) top = fmaxf(top, sv[u]);
             }
-            float t0 = sv[32 * h], t1 = sv[32 * h + 1];
+            const float next = fmaxf(m, top * c);
+            const float f = next > m ? exp2f(m - next) : 1.f;  // 0 for the row's first visible key
+            m = next;
+            sum[0].x *= f, sum[0].y *= f, sum[1].x *= f, sum[1].y *= f;
+            if (n > 0) {  // the products before this S have completed: O is this warp's to change
+#pragma unroll 1
+              for (int h = 0; h < DP / 16; ++h) {
+                uint32_t o[16];
+                tmem_ld16(tO + 16 * h, o);
 #pragma unroll
-            for (int u = 2; u < 32; u += 2) t0 = fmaxf(t0, sv[32 * h + u]), t1 = fmaxf(t1, sv[32 * h + u + 1]);
-            top = fmaxf(top, fmaxf(t0, t1));
-          }
-        }
-        top *= c;
-        const bool raise = top > m + 8.f;
-        if (__any_sync(0xffffffffu, raise)) {
-          const float f = raise ? exp2f(m - top) : 1.f;  // 0 for the row's first visible key
-          if (raise) m = top;
-          sum[0].x *= f, sum[0].y *= f, sum[1].x *= f, sum[1].y *= f;
-          if (n > 0) {  // the products before this S have completed: O is this warp's to change
-#pragma unroll
-            for (int h = 0; h < DP / 32; ++h) {
-              float o[32];
-              tmem_ld32(tO + 32 * h, o);
-              uint32_t w[16];
-#pragma unroll
-              for (int part = 0; part < 2; ++part) {
-#pragma unroll
-                for (int u = 0; u < 16; ++u) w[u] = __float_as_uint(o[16 * part + u] * f);
-                tmem_st16(tO + 32 * h + 16 * part, w);
+                for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
+                tmem_st16(tO + 16 * h, o);
               }
             }
           }
-        }
-        const float off = m == -INFINITY ? 0.f : -m;
-        const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
+          const float off = m == -INFINITY ? 0.f : -m;
+          const float2 off2 = make_float2(off, off);
+          t2[0] = t2[1] = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int h = 0; h < KT / 32; ++h) {
-          uint32_t w[16];
-          if (none >> h & 1) {
+          for (int h = 0; h < KT / 32; ++h) {
+            const int kc = k0 + 32 * h;
+            if (window_none(qlo, qhi, kc, kc + 31, p.window, p.sinks)) {
 #pragma unroll
-            for (int u = 0; u < 16; ++u) w[u] = 0u;
-          } else {
+              for (int u = 0; u < 16; ++u) w[16 * h + u] = 0u;
+              continue;
+            }
+            float sv[32];
+            tmem_read32(tS + 32 * h, sv);
+            if (!window_all(qlo, qhi, kc, kc + 31, p.window, p.sinks)) {
+#pragma unroll
+              for (int u = 0; u < 32; ++u)
+                if (!window_sees(q, kc + u, p.window, p.sinks)) sv[u] = -INFINITY;
+            }
 #pragma unroll
             for (int u = 0; u < 16; ++u) {
-              const float2 x = __ffma2_rn(make_float2(sv[32 * h + 2 * u], sv[32 * h + 2 * u + 1]), c2, off2);
+              const float2 x = __ffma2_rn(make_float2(sv[2 * u], sv[2 * u + 1]), c2, off2);
               const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-              sum[u & 1] = __fadd2_rn(sum[u & 1], e);
-              w[u] = pack2<E>(e.x, e.y);
+              t2[u & 1] = __fadd2_rn(t2[u & 1], e);
+              w[16 * h + u] = pack2<E>(e.x, e.y);
             }
           }
-          tmem_st16(tS + 16 * h, w);
+          if (raise) break;
+          const float t = (t2[0].x + t2[0].y) + (t2[1].x + t2[1].y);
+          if (__all_sync(0xffffffffu, t <= kWinTileSum)) break;
+          raise = true;
         }
+        sum[0] = __fadd2_rn(sum[0], t2[0]), sum[1] = __fadd2_rn(sum[1], t2[1]);
+#pragma unroll
+        for (int h = 0; h < KT / 32; ++h) tmem_st16(tS + 16 * h, *reinterpret_cast<uint32_t(*)[16]>(w + 16 * h));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -337,7 +342,7 @@ __global__ void __launch_bounds__(WinFwd<DP>::kThreads, WinFwd<DP>::kCtas)
 #pragma unroll
         for (int h = 0; h < DP / 32; ++h) {
           float o[32];
-          tmem_ld32(tO + 32 * h, o);
+          tmem_read32(tO + 32 * h, o);
           if (i >= p.Tq) continue;
 #pragma unroll
           for (int u = 0; u < 4; ++u) {

@@ -17,8 +17,10 @@
 //   P and dS, as 16-bit pairs over the columns that S and dP lay in, are the A operands of
 //   keys' side (X = K, V; Y = Q, dO; rows are keys):     dV += P Y1, dK += dS Y0
 //   queries' side (X = Q, dO; Y = K, V; rows are queries): dQ += dS Y0
-// with Y0, Y1 read a second time, now as MN-major B operands, from the same shared memory. Two buffers of S and dP,
-// each with its own group of four warps, let one item's products run while the other's exponentials do.
+// with Y0, Y1 read a second time, now as MN-major B operands, from the same shared memory. What bounds the kernel is
+// each item's chain (S and dP, the warps' arithmetic, the gradients' products), not a unit, so two items are in
+// flight per SM (two CTAs with one buffer of S and dP each at a head width of 64, one CTA with two buffers at 128)
+// and eight warps share an item, each with 32 rows and half of the columns.
 // P and dS are rounded to bf16, as the tensor core needs; sums are fp32.
 //
 // Sinks are seen by every later query, so their key tiles have far more work than the others: it is dealt in
@@ -41,14 +43,17 @@ struct WindowGrad {
 
 template <int DP>
 struct WinBwd {
-  static constexpr int kX = 128, kY = 64, NB = 2, YS = 3;
-  static constexpr int kThreads = (2 + 4 * NB) * 32;
+  static constexpr int kX = 128, kY = 64, YS = 3;
+  static constexpr int NB = DP == 64 ? 1 : 2, kCtas = DP == 64 ? 2 : 1;
+  static constexpr int kSets = 2 * NB;  // sets of four warps: each buffer's columns are shared by two
+  static constexpr int kThreads = (2 + 4 * kSets) * 32;
   static constexpr int kXBytes = kX * DP * 2, kYBytes = kY * DP * 2, kStatBytes = 512;
   static constexpr int kStage = 2 * kYBytes;
   static constexpr int kCore = 2 * kXBytes + YS * kStage;
   static constexpr int kSmem = 1024 + kCore + YS * kStatBytes + 256;
   static constexpr uint32_t kAcc = NB * 128;  // columns: NB x (S 64, dP 64), then the gradients
-  static constexpr uint32_t kTmemCols = 512;
+  static constexpr uint32_t kTmemCols = 512 / kCtas;
+  static_assert(kAcc + 2 * DP <= kTmemCols, "S, dP and both gradients lie in tensor memory");
 };
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -90,7 +95,7 @@ __global__ void __launch_bounds__(256) window_stats_kernel(const __nv_bfloat16* 
 }
 
 template <int DP, bool kKeys>
-__global__ void __launch_bounds__(WinBwd<DP>::kThreads, 1)
+__global__ void __launch_bounds__(WinBwd<DP>::kThreads, WinBwd<DP>::kCtas)
     window_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __grid_constant__ CUtensorMap tm_x1,
                            const __grid_constant__ CUtensorMap tm_y0, const __grid_constant__ CUtensorMap tm_y1,
                            const __grid_constant__ WindowGrad p) {
@@ -143,12 +148,18 @@ __global__ void __launch_bounds__(WinBwd<DP>::kThreads, 1)
       items = sink_y + q_last / kY - first_y + 1;
     }
   }
-  // item t: its Y tile and the query head it belongs to
-  auto y_tile = [&](int t) {
-    if (kKeys) return first_y + (begin + t) % per_head;
-    return t < sink_y ? t : first_y + t - sink_y;
+  // A walk over the items: the Y tile and, on the keys' side, the query head of the item it stands at.
+  struct Walk {
+    int y, head;
   };
-  auto item_head = [&](int t) { return kKeys ? head0 + (begin + t) / per_head : head0; };
+  auto step_to = [&](Walk& it, int t, int n) {  // n items further, to item t
+    if (kKeys) {
+      for (it.y += n; it.y >= first_y + per_head; it.y -= per_head) ++it.head;
+    } else {
+      it.y = t < sink_y ? t : first_y + t - sink_y;
+    }
+  };
+  Walk it{first_y, kKeys ? head0 : 0};
 
   __nv_bfloat16* g0 = reinterpret_cast<__nv_bfloat16*>(kKeys ? p.dk : p.dq);
   __nv_bfloat16* g1 = reinterpret_cast<__nv_bfloat16*>(p.dv);
@@ -188,7 +199,7 @@ __global__ void __launch_bounds__(WinBwd<DP>::kThreads, 1)
   if (tid == 0) {
     mbar_init(x_full, 1);
     for (int s = 0; s < YS; ++s) mbar_init(&y_full[s], 1), mbar_init(&y_empty[s], 1);
-    for (int s = 0; s < NB; ++s) mbar_init(&s_full[s], 1), mbar_init(&p_full[s], 4);
+    for (int s = 0; s < NB; ++s) mbar_init(&s_full[s], 1), mbar_init(&p_full[s], 8);
     mbar_init(tail, 1);
     mbar_init(done, 1);
     *abort_flag = 0;
@@ -220,7 +231,8 @@ __global__ void __launch_bounds__(WinBwd<DP>::kThreads, 1)
     const int end = kKeys ? rows : length, total = kKeys ? w.Tq : w.Tk;
     int t = 0, tails = 0;
     for (; t < items; ++t) {
-      const int st = t % YS, y0 = y_tile(t) * kY, hd = kKeys ? item_head(t) : kv;
+      step_to(it, t, t == 0 ? begin : 1);
+      const int st = t % YS, y0 = it.y * kY, hd = kKeys ? it.head : kv;
       if (!all_lanes(mbar_wait(&y_empty[st], ((t / YS) & 1) ^ 1, abort_flag, status))) break;
       const int behind = y0 + kY - end;
       const bool clear = behind > 0 && end < total;
@@ -282,15 +294,16 @@ __global__ void __launch_bounds__(WinBwd<DP>::kThreads, 1)
           if (!(ok = mbar_wait(&p_full[bf], (u / NB) & 1, abort_flag, status))) break;
           tc_fence_after();
           const uint32_t tP = tmem + 128 * bf, tD = tP + 64;
+          auto half = [](int k) { return 8 * k + (k < kY / 32 ? 0 : 16); };  // columns of P for query or key 16 k
           const uint64_t d0 = smem_desc_sw128_mn(sY + st * L::kStage, kY * 128);
           const uint64_t d1 = smem_desc_sw128_mn(sY + st * L::kStage + L::kYBytes, kY * 128);
 #pragma unroll
           for (int k = 0; k < kY / 16; ++k)
-            tc_mma_f16_ts(tmem + L::kAcc, tD + 8 * k, d0 + (uint64_t)(2048 >> 4) * k, idesc_g, (u > 0 || k > 0) ? 1u : 0u);
+            tc_mma_f16_ts(tmem + L::kAcc, tD + half(k), d0 + (uint64_t)(2048 >> 4) * k, idesc_g, (u > 0 || k > 0) ? 1u : 0u);
           if (kKeys) {
 #pragma unroll
             for (int k = 0; k < kY / 16; ++k)
-              tc_mma_f16_ts(tmem + L::kAcc + DP, tP + 8 * k, d1 + (uint64_t)(2048 >> 4) * k, idesc_g,
+              tc_mma_f16_ts(tmem + L::kAcc + DP, tP + half(k), d1 + (uint64_t)(2048 >> 4) * k, idesc_g,
                             (u > 0 || k > 0) ? 1u : 0u);
           }
           tc_commit(&y_empty[st]);
@@ -302,72 +315,78 @@ __global__ void __launch_bounds__(WinBwd<DP>::kThreads, 1)
     __syncwarp();
   } else {
     // ---------------- P and dS, then the gradients out ----------------
-    const int bf = (warp - 2) >> 2, quarter = warp & 3;
+    const int set = (warp - 2) >> 2, bf = set >> 1, h = set & 1, quarter = warp & 3;  // h: half of the columns
     const int r = x0 + quarter * 32 + lane;  // this thread's row of X: a key, or a query row
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tS = tmem + 128 * bf + lanes, tD = tS + 64;
+    const uint32_t tS = tmem + 128 * bf + lanes, tD = tS + 64;  // S and P, dP and dS
     const float c = w.scale * 1.4426950408889634f;
     const float2 c2 = make_float2(c, c);
     const int rlo = x0 + quarter * 32, rhi = rlo + 31;
-    float2 nl = make_float2(0.f, 0.f), nd = nl;
+    // -lse and -Delta, of the row (queries' side, in the first two places) or of four columns
+    float4 nl4 = make_float4(0.f, 0.f, 0.f, 0.f), nd4 = nl4;
     if (!kKeys) {
       const float* st = p.stat + (((int64_t)b * w.H + head0) * p.stat_tiles + r / kY) * 128 + r % kY;
       const bool have = r < p.stat_tiles * kY;
-      const float l = have ? __ldg(st) : -INFINITY, d = have ? __ldg(st + 64) : 0.f;
-      nl = make_float2(l, l), nd = make_float2(d, d);
+      nl4.x = nl4.y = have ? __ldg(st) : -INFINITY, nd4.x = nd4.y = have ? __ldg(st + 64) : 0.f;
     }
     bool ok = true;
     for (int t = bf; t < items; t += NB) {
-      const int st = t % YS, y0 = y_tile(t) * kY;
+      step_to(it, t, t == bf ? begin + bf : NB);
+      const int st = t % YS, y0 = it.y * kY;
       // keys' side: the columns' statistics arrive with the tile
       if (kKeys && !(ok = mbar_wait(&y_full[st], (t / YS) & 1, abort_flag, status))) break;
       if (!(ok = mbar_wait(&s_full[bf], (t / NB) & 1, abort_flag, status))) break;
       tc_fence_after();
       const float* stat = sStat + st * 128;
+      const int yc = y0 + 32 * h;
+      const int qlo = kKeys ? w.offset + yc : w.offset + rlo, qhi = kKeys ? qlo + 31 : w.offset + rhi;
+      const int klo = kKeys ? rlo : yc, khi = kKeys ? rhi : yc + 31;
+      uint32_t pw[16], dw[16];
+      const bool none = window_none(qlo, qhi, klo, khi, w.window, w.sinks);
+      if (none) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int yc = y0 + 32 * h;
-        const int qlo = kKeys ? w.offset + yc : w.offset + rlo, qhi = kKeys ? qlo + 31 : w.offset + rhi;
-        const int klo = kKeys ? rlo : yc, khi = kKeys ? rhi : yc + 31;
-        uint32_t pw[16], dw[16];
-        if (window_none(qlo, qhi, klo, khi, w.window, w.sinks)) {
+        for (int u = 0; u < 16; ++u) pw[u] = dw[u] = 0u;
+      } else {
+        uint32_t s[32], d[32];
+        tmem_ld32_async(tS + 32 * h, s);
+        tmem_ld32_async(tD + 32 * h, d);
+        tmem_wait_ld_regs(s);
+        tmem_wait_ld_regs(d);
+        // visible pairs, bit by column; keys past the end of a padded sequence lie behind every query with a token
+        uint32_t seen = 0xffffffffu;
+        if (!window_all(qlo, qhi, klo, khi, w.window, w.sinks)) {
+          seen = 0u;
 #pragma unroll
-          for (int u = 0; u < 16; ++u) pw[u] = dw[u] = 0u;
-        } else {
-          uint32_t s[32], d[32];
-          tmem_ld32_async(tS + 32 * h, s);
-          tmem_ld32_async(tD + 32 * h, d);
-          tmem_wait_ld_regs(s);
-          tmem_wait_ld_regs(d);
-          // keys past the end of a padded sequence lie behind every query with a token: never "all"
-          const bool all = window_all(qlo, qhi, klo, khi, w.window, w.sinks);
+          for (int u = 0; u < 32; ++u)
+            if (kKeys ? window_sees(w.offset + yc + u, r, w.window, w.sinks)
+                      : window_sees(w.offset + r, yc + u, w.window, w.sinks))
+              seen |= 1u << u;
+        }
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          if (kKeys && (u & 1) == 0) {
+            nl4 = *reinterpret_cast<const float4*>(stat + 32 * h + 2 * u);
+            nd4 = *reinterpret_cast<const float4*>(stat + 64 + 32 * h + 2 * u);
+          }
+          const float2 nl = kKeys && (u & 1) ? make_float2(nl4.z, nl4.w) : make_float2(nl4.x, nl4.y);
+          const float2 nd = kKeys && (u & 1) ? make_float2(nd4.z, nd4.w) : make_float2(nd4.x, nd4.y);
+          const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * u]), __uint_as_float(s[2 * u + 1])), c2, nl);
+          const float2 pr = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+          const float2 e = __fadd2_rn(make_float2(__uint_as_float(d[2 * u]), __uint_as_float(d[2 * u + 1])), nd);
+          const float2 ds = __fmul2_rn(pr, e);
+          pw[u] = pack2<__nv_bfloat16>(pr.x, pr.y);
+          dw[u] = pack2<__nv_bfloat16>(ds.x, ds.y);
+        }
+        if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {  // clear what is hidden, whatever it came to
 #pragma unroll
           for (int u = 0; u < 16; ++u) {
-            if (kKeys) {
-              nl = *reinterpret_cast<const float2*>(stat + 32 * h + 2 * u);
-              nd = *reinterpret_cast<const float2*>(stat + 64 + 32 * h + 2 * u);
-            }
-            const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * u]), __uint_as_float(s[2 * u + 1])), c2, nl);
-            float2 pr = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-            const float2 e = __fadd2_rn(make_float2(__uint_as_float(d[2 * u]), __uint_as_float(d[2 * u + 1])), nd);
-            float2 ds = __fmul2_rn(pr, e);
-            if (!all) {
-              const int y = yc + 2 * u;
-              const bool a0 = kKeys ? window_sees(w.offset + y, r, w.window, w.sinks)
-                                    : window_sees(w.offset + r, y, w.window, w.sinks);
-              const bool a1 = kKeys ? window_sees(w.offset + y + 1, r, w.window, w.sinks)
-                                    : window_sees(w.offset + r, y + 1, w.window, w.sinks);
-              pr.x = a0 ? pr.x : 0.f, ds.x = a0 ? ds.x : 0.f;
-              pr.y = a1 ? pr.y : 0.f, ds.y = a1 ? ds.y : 0.f;
-            }
-            pw[u] = pack2<__nv_bfloat16>(pr.x, pr.y);
-            dw[u] = pack2<__nv_bfloat16>(ds.x, ds.y);
+            const uint32_t two = seen >> (2 * u), keep = (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+            pw[u] &= keep, dw[u] &= keep;
           }
         }
-        // columns 16h .. of S and dP have been read by this half or the one before
-        if (kKeys) tmem_st16(tS + 16 * h, pw);
-        tmem_st16(tD + 16 * h, dw);
       }
+      if (kKeys) tmem_st16(tS + 32 * h, pw);  // over the half of S, and of dP, that this warp has read
+      tmem_st16(tD + 32 * h, dw);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -375,17 +394,18 @@ __global__ void __launch_bounds__(WinBwd<DP>::kThreads, 1)
     }
     if (ok && mbar_wait(done, 0, abort_flag, status)) {
       tc_fence_after();
-      // keys' side: group 0 writes dK, group 1 dV; queries' side: the groups share dQ's columns
-      const bool first = bf == 0;
-      const float f = kKeys && !first ? 1.f : w.scale;
-      __nv_bfloat16* g = kKeys && !first ? g1 : g0;
-      const uint32_t tG = tmem + L::kAcc + lanes + (kKeys && !first ? DP : 0);
       const bool have = kKeys ? r < length : r < rows;
+      // the gradients' 32-column chunks (keys' side: dK's, then dV's) go round the sets
 #pragma unroll
-      for (int h = 0; h < DP / 32; ++h) {
-        if (!kKeys && (h & 1) != bf) continue;
+      for (int k = 0; k < (kKeys ? 2 : 1) * (DP / 32); ++k) {
+        if (k % L::kSets != set) continue;
+        const bool first = k < DP / 32;
+        const int h = first ? k : k - DP / 32;
+        const float f = first ? w.scale : 1.f;
+        __nv_bfloat16* g = first ? g0 : g1;
+        const uint32_t tG = tmem + L::kAcc + lanes + (first ? 0 : DP);
         float o[32];
-        tmem_ld32(tG + 32 * h, o);
+        tmem_read32(tG + 32 * h, o);
         if (slot >= 0) {
           float* out = p.partial + (((int64_t)slot * 2 + (first ? 0 : 1)) * kX + (r - x0)) * w.D + 32 * h;
 #pragma unroll
