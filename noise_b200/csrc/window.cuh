@@ -21,17 +21,29 @@ __device__ __forceinline__ int window_length(const WindowParams& p, int b) {
   return p.lengths ? min(max(__ldg(p.lengths + b), 0), p.Tk) : p.Tk;
 }
 
-// Query at position q sees key k.
-__device__ __forceinline__ bool window_sees(int q, int k, int window, int sinks) {
-  return k <= q && (q - k <= window || k < sinks);
-}
-
 // Queries qlo .. qhi against keys klo .. khi: no pair visible, or every pair.
 __device__ __forceinline__ bool window_none(int qlo, int qhi, int klo, int khi, int window, int sinks) {
   return klo > qhi || (qlo - khi > window && klo >= sinks);
 }
 __device__ __forceinline__ bool window_all(int qlo, int qhi, int klo, int khi, int window, int sinks) {
   return khi <= qlo && (qhi - klo <= window || khi < sinks);
+}
+
+// The low n bits (n clamped to [0, 32]).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  uint32_t r;
+  asm("bmsk.clamp.b32 %0, 0, %1;" : "=r"(r) : "r"(max(n, 0)));
+  return r;
+}
+
+// Bit u: query q sees key k0 + u (u < 32).
+__device__ __forceinline__ uint32_t window_keys(int q, int k0, int window, int sinks) {
+  return low_bits(q - k0 + 1) & (~low_bits(q - window - k0) | low_bits(sinks - k0));
+}
+
+// Bit u: query q0 + u sees key k (u < 32).
+__device__ __forceinline__ uint32_t window_queries(int q0, int k, int window, int sinks) {
+  return ~low_bits(k - q0) & (k < sinks ? 0xffffffffu : low_bits(k + window - q0 + 1));
 }
 
 // 32 columns of this warp's tensor memory lanes; the wait names the registers, so that no use moves before it.

@@ -6,19 +6,27 @@
 // One pass over the keys: each query row keeps a reference m and the sum l of exp(S - m). m is the maximum of
 // the first tile the row sees, and is raised only when a later tile's P sums to more than 2^10 under it; then
 // the tile is taken again under its new maximum and O (in tensor memory) and l are scaled by exp(m_old - m_new).
-// The sum that l needs anyway thus guards the range, and the usual tile spends no instruction on a maximum:
-// 153 -> FWD us at B 8, T 2048, 8 heads of 64, window 1024, 4 sinks. P, l and O only meet as P / l and O / l, so
-// a reference below the maximum costs no accuracy.
+// The sum that l needs anyway thus guards the range, and the usual tile spends no instruction on a maximum. P, l
+// and O only meet as P / l and O / l, so a reference below the maximum costs no accuracy.
 //
 // One CTA = two consecutive tiles of 128 queries of one head; they share every key and value tile the CTA
 // streams, while one tile's products overlap the other's exponentials. Key tiles: the sinks' first, then
-// those the window reaches; 32 x 32 blocks of scores are skipped, taken without masks, or masked per key.
+// those the window reaches; 32 x 32 blocks of scores are skipped, taken without masks, or masked by a word of
+// visible keys.
 //   warp 0       TMA producer: Q once, then K and V tiles on rings of their own
 //   warp 1       tensor memory owner and MMA issuer: per key tile and query tile, O += P V of the tile before,
 //                then S = Q K^T (S reuses the columns that P lay in)
 //   warps 2 ..   one query row a thread: S from tensor memory, the softmax step, P back over S as 16-bit pairs
 // The head width is padded to 64 or 128 by the tensor maps' zero fill. At 64 (key tiles of 64, 256 columns of
 // tensor memory) two CTAs share an SM; at 128 (key tiles of 128) one CTA takes all 512 columns.
+//
+// Measured at B 8, T 2048, 8 heads of 64, window 1024, 4 sinks (bf16) and at T 16384, 16 heads on 4 key heads of
+// 128, window 4096, 64 sinks (fp16): 76 and 504 us. The bound is the chain S -> softmax -> P -> O of each tile and
+// the products' rate: without any softmax work the same pipeline takes 53 and 377 us, and the products alone 31 and
+// 305 us at their measured rates (43 + N / 2 cycles for 16 values of the inner dimension with both operands in
+// shared memory, 11 + N / 2 with A in tensor memory). A maximum of every tile costs 153 against 102 us (with
+// the products issued from a one-lane branch); P in columns of its own beside S, which frees S earlier but leaves one CTA an
+// SM at 64, 84 and 551 us.
 // P is rounded to the input type, as the tensor core needs it; the row sum is of the unrounded values.
 //
 // A key tile that crosses the end of a padded sequence is loaded apart: the producer warp clears the value
@@ -187,53 +195,63 @@ __global__ void __launch_bounds__(WinFwd<DP>::kThreads, WinFwd<DP>::kCtas)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ---------------- MMA issuer ----------------
-      const uint32_t idesc_s = make_idesc(kFmt, kQ, KT);
-      const uint32_t idesc_o = make_idesc(kFmt, kQ, DP, 0, 1);  // B = V is MN-major
-      int np[G] = {0, 0};  // PV products issued
-      bool ok = mbar_wait(q_full, 0, abort_flag, status);
-      tc_fence_after();
-      for (int t = 0; ok && t <= walk.n; ++t) {
-        const int pt = t - 1;
-        bool v_ready = false, k_ready = false;
+    // ---------------- MMA issuer ----------------
+    // The whole warp walks the loop, so that descriptors and addresses are warp-uniform values; one elected lane
+    // issues. (From inside a one-lane branch every product waits for its operands to reach uniform registers,
+    // about 100 cycles.)
+    const uint32_t idesc_s = make_idesc(kFmt, kQ, KT);
+    const uint32_t idesc_o = make_idesc(kFmt, kQ, DP, 0, 1);  // B = V is MN-major
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const bool issuer = elect_one();
+    int np[G] = {0, 0};                                       // PV products issued
+    bool need[G] = {false, false};                            // which query tiles the tile before is for
+    bool ok = mbar_wait_warp(q_full, 0, abort_flag, status);
+    for (int t = 0; ok && t <= walk.n; ++t) {
+      bool now[G] = {false, false};
+      const int ks = t % KS, vs = (t + VS - 1) % VS;  // stages of this tile's keys and the last tile's values
+      if (t < walk.n) {
+        const int kt = walk.tile(t);
+        now[0] = needs(0, kt), now[1] = active > 1 && needs(1, kt);
+        if (!(ok = mbar_wait_warp(&k_full[ks], (t / KS) & 1, abort_flag, status))) break;
+      }
+      if (t > 0 && !(ok = mbar_wait_warp(&v_full[vs], ((t - 1) / VS) & 1, abort_flag, status))) break;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          if (!ok || g >= active) continue;
-          const uint32_t tS = tmem + L::kGroupCols * g, tO = tS + KT;
-          if (pt >= 0 && needs(g, walk.tile(pt))) {
-            if (!v_ready) ok = v_ready = mbar_wait(&v_full[pt % VS], (pt / VS) & 1, abort_flag, status);
-            if (ok) ok = mbar_wait(&p_full[g], np[g] & 1, abort_flag, status);
-            if (!ok) continue;
+      for (int g = 0; g < G; ++g) {
+        const uint32_t tS = tm + L::kGroupCols * g;
+        if (ok && need[g]) {
+          ok = mbar_wait_warp(&p_full[g], np[g] & 1, abort_flag, status);
+          if (ok) {
             tc_fence_after();
-            const uint64_t dv = smem_desc_sw128_mn(sV + (pt % VS) * L::kTileBytes, KT * 128);
+            if (issuer) {
+              const uint64_t dv = smem_desc_sw128_mn(sV + vs * L::kTileBytes, KT * 128);
 #pragma unroll
-            for (int k = 0; k < KT / 16; ++k)
-              tc_mma_f16_ts(tO, tS + 8 * k, dv + (uint64_t)(2048 >> 4) * k, idesc_o, (np[g] > 0 || k > 0) ? 1u : 0u);
+              for (int k = 0; k < KT / 16; ++k)
+                tc_mma_f16_ts(tS + KT, tS + 8 * k, dv + (uint64_t)(2048 >> 4) * k, idesc_o, (np[g] > 0 || k > 0) ? 1u : 0u);
+              if (walk.tile(t - 1) == (g ? hi1 : hi0)) tc_commit(&o_full[g]);
+            }
             ++np[g];
-            if (walk.tile(pt) == (g ? hi1 : hi0)) tc_commit(&o_full[g]);
           }
-          if (t < walk.n && needs(g, walk.tile(t))) {
-            if (!k_ready) {
-              ok = k_ready = mbar_wait(&k_full[t % KS], (t / KS) & 1, abort_flag, status);
-              if (!ok) continue;
-              tc_fence_after();
-            }
-            const uint8_t* kt_base = sK + (t % KS) * L::kTileBytes;
-            const uint8_t* q_base = sQ + g * L::kQBytes;
+        }
+        if (ok && now[g]) {
+          tc_fence_after();
+          if (issuer) {
+            const uint64_t dq = smem_desc_sw128(sQ + g * L::kQBytes), dk = smem_desc_sw128(sK + ks * L::kTileBytes);
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-              const uint64_t dq = smem_desc_sw128(q_base + (k / 4) * (kQ * 128)) + 2 * (k % 4);
-              const uint64_t dk = smem_desc_sw128(kt_base + (k / 4) * (KT * 128)) + 2 * (k % 4);
-              tc_mma_f16(tS, dq, dk, idesc_s, k > 0 ? 1u : 0u);
-            }
+            for (int k = 0; k < DP / 16; ++k)
+              tc_mma_f16(tS, dq + (k / 4) * (kQ * 128 >> 4) + 2 * (k % 4),
+                         dk + (k / 4) * (KT * 128 >> 4) + 2 * (k % 4), idesc_s, k > 0 ? 1u : 0u);
             tc_commit(&s_full[g]);
           }
         }
-        if (!ok) break;
-        if (pt >= 0) tc_commit(&v_empty[pt % VS]);
-        if (t < walk.n) tc_commit(&k_empty[t % KS]);
       }
+      if (!ok) break;
+      if (issuer) {
+        if (t > 0) tc_commit(&v_empty[vs]);
+        if (t < walk.n) tc_commit(&k_empty[ks]);
+      }
+      need[0] = now[0], need[1] = now[1];
+    }
+    if (issuer) {
       tc_commit(drain);
       mbar_wait(drain, 0, abort_flag, status);
     }
@@ -275,9 +293,10 @@ __global__ void __launch_bounds__(WinFwd<DP>::kThreads, WinFwd<DP>::kCtas)
               if (window_none(qlo, qhi, kc, kc + 31, p.window, p.sinks)) continue;
               float sv[32];
               tmem_read32(tS + 32 * h, sv);
+              const uint32_t seen = window_keys(q, kc, p.window, p.sinks);
 #pragma unroll
               for (int u = 0; u < 32; ++u)
-                if (window_sees(q, kc + u, p.window, p.sinks)) top = fmaxf(top, sv[u]);
+                if (seen >> u & 1) top = fmaxf(top, sv[u]);
             }
             const float next = fmaxf(m, top * c);
             const float f = next > m ? exp2f(m - next) : 1.f;  // 0 for the row's first visible key
@@ -308,9 +327,10 @@ __global__ void __launch_bounds__(WinFwd<DP>::kThreads, WinFwd<DP>::kCtas)
             float sv[32];
             tmem_read32(tS + 32 * h, sv);
             if (!window_all(qlo, qhi, kc, kc + 31, p.window, p.sinks)) {
+              const uint32_t seen = window_keys(q, kc, p.window, p.sinks);
 #pragma unroll
               for (int u = 0; u < 32; ++u)
-                if (!window_sees(q, kc + u, p.window, p.sinks)) sv[u] = -INFINITY;
+                if (!(seen >> u & 1)) sv[u] = -INFINITY;
             }
 #pragma unroll
             for (int u = 0; u < 16; ++u) {

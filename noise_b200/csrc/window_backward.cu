@@ -265,50 +265,56 @@ __global__ void __launch_bounds__(WinBwd<DP>::kThreads, WinBwd<DP>::kCtas)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ---------------- MMA issuer ----------------
-      // Item t's S and dP, then the gradients of item t - 1: with two buffers, S(t) overwrites the
-      // columns of P(t - 2), whose products were issued before it.
-      const uint32_t idesc_s = make_idesc(1, kX, kY), idesc_g = make_idesc(1, kX, DP, 0, 1);
-      bool ok = mbar_wait(x_full, 0, abort_flag, status);
-      for (int t = 0; ok && t < items + NB - 1; ++t) {
-        if (t < items) {
-          const int st = t % YS, bf = t % NB;
-          if (!(ok = mbar_wait(&y_full[st], (t / YS) & 1, abort_flag, status))) break;
-          tc_fence_after();
-          const uint8_t* y = sY + st * L::kStage;
-          const uint32_t tS = tmem + 128 * bf;
+    // ---------------- MMA issuer (the whole warp, one elected lane issuing: see the forward) ----------------
+    // Item t's S and dP, then the gradients of item t - 1: with two buffers, S(t) overwrites the
+    // columns of P(t - 2), whose products were issued before it.
+    const uint32_t idesc_s = make_idesc(1, kX, kY), idesc_g = make_idesc(1, kX, DP, 0, 1);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const bool issuer = elect_one();
+    bool ok = mbar_wait_warp(x_full, 0, abort_flag, status);
+    for (int t = 0; ok && t < items + NB - 1; ++t) {
+      if (t < items) {
+        const int st = t % YS, bf = t % NB;
+        if (!(ok = mbar_wait_warp(&y_full[st], (t / YS) & 1, abort_flag, status))) break;
+        tc_fence_after();
+        const uint32_t tS = tm + 128 * bf;
+        if (issuer) {
+          const uint64_t x = smem_desc_sw128(sX), y = smem_desc_sw128(sY + st * L::kStage);
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k)
-            tc_mma_f16(tS, smem_desc_sw128(sX + (k / 4) * (kX * 128)) + 2 * (k % 4),
-                       smem_desc_sw128(y + (k / 4) * (kY * 128)) + 2 * (k % 4), idesc_s, k > 0 ? 1u : 0u);
+            tc_mma_f16(tS, x + (k / 4) * (kX * 128 >> 4) + 2 * (k % 4), y + (k / 4) * (kY * 128 >> 4) + 2 * (k % 4), idesc_s,
+                       k > 0 ? 1u : 0u);
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k)
-            tc_mma_f16(tS + 64, smem_desc_sw128(sX + L::kXBytes + (k / 4) * (kX * 128)) + 2 * (k % 4),
-                       smem_desc_sw128(y + L::kYBytes + (k / 4) * (kY * 128)) + 2 * (k % 4), idesc_s, k > 0 ? 1u : 0u);
+            tc_mma_f16(tS + 64, x + (L::kXBytes >> 4) + (k / 4) * (kX * 128 >> 4) + 2 * (k % 4),
+                       y + (L::kYBytes >> 4) + (k / 4) * (kY * 128 >> 4) + 2 * (k % 4), idesc_s, k > 0 ? 1u : 0u);
           tc_commit(&s_full[bf]);
         }
-        const int u = t - (NB - 1);
-        if (u >= 0) {
-          const int st = u % YS, bf = u % NB;
-          if (!(ok = mbar_wait(&p_full[bf], (u / NB) & 1, abort_flag, status))) break;
-          tc_fence_after();
-          const uint32_t tP = tmem + 128 * bf, tD = tP + 64;
-          auto half = [](int k) { return 8 * k + (k < kY / 32 ? 0 : 16); };  // columns of P for query or key 16 k
+      }
+      const int u = t - (NB - 1);
+      if (u >= 0) {
+        const int st = u % YS, bf = u % NB;
+        if (!(ok = mbar_wait_warp(&p_full[bf], (u / NB) & 1, abort_flag, status))) break;
+        tc_fence_after();
+        const uint32_t tP = tm + 128 * bf, tD = tP + 64;
+        auto half = [](int k) { return 8 * k + (k < kY / 32 ? 0 : 16); };  // columns of P for query or key 16 k
+        if (issuer) {
           const uint64_t d0 = smem_desc_sw128_mn(sY + st * L::kStage, kY * 128);
-          const uint64_t d1 = smem_desc_sw128_mn(sY + st * L::kStage + L::kYBytes, kY * 128);
+          const uint64_t d1 = d0 + (L::kYBytes >> 4);
 #pragma unroll
           for (int k = 0; k < kY / 16; ++k)
-            tc_mma_f16_ts(tmem + L::kAcc, tD + half(k), d0 + (uint64_t)(2048 >> 4) * k, idesc_g, (u > 0 || k > 0) ? 1u : 0u);
+            tc_mma_f16_ts(tm + L::kAcc, tD + half(k), d0 + (uint64_t)(2048 >> 4) * k, idesc_g, (u > 0 || k > 0) ? 1u : 0u);
           if (kKeys) {
 #pragma unroll
             for (int k = 0; k < kY / 16; ++k)
-              tc_mma_f16_ts(tmem + L::kAcc + DP, tP + half(k), d1 + (uint64_t)(2048 >> 4) * k, idesc_g,
+              tc_mma_f16_ts(tm + L::kAcc + DP, tP + half(k), d1 + (uint64_t)(2048 >> 4) * k, idesc_g,
                             (u > 0 || k > 0) ? 1u : 0u);
           }
           tc_commit(&y_empty[st]);
         }
       }
+    }
+    if (issuer) {
       tc_commit(done);
       mbar_wait(done, 0, abort_flag, status);
     }
@@ -355,12 +361,7 @@ __global__ void __launch_bounds__(WinBwd<DP>::kThreads, WinBwd<DP>::kCtas)
         // visible pairs, bit by column; keys past the end of a padded sequence lie behind every query with a token
         uint32_t seen = 0xffffffffu;
         if (!window_all(qlo, qhi, klo, khi, w.window, w.sinks)) {
-          seen = 0u;
-#pragma unroll
-          for (int u = 0; u < 32; ++u)
-            if (kKeys ? window_sees(w.offset + yc + u, r, w.window, w.sinks)
-                      : window_sees(w.offset + r, yc + u, w.window, w.sinks))
-              seen |= 1u << u;
+          seen = kKeys ? window_queries(qlo, r, w.window, w.sinks) : window_keys(w.offset + r, yc, w.window, w.sinks);
         }
 #pragma unroll
         for (int u = 0; u < 16; ++u) {
