@@ -55,6 +55,23 @@ __device__ __forceinline__ void tmem_read32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// The order in which CTAs take (tile, sequence and head) pairs: heavy tiles first, over groups of pairs whose
+// streamed operands fit the L2 cache together, so that the last CTAs to run are short ones.
+struct TileOrder {
+  int tiles, pairs, group;  // pairs: sequences x heads
+  __device__ __forceinline__ void at(int index, int& tile, int& pair) const {
+    const int full = tiles * group, g = index / full, rest = index - g * full;
+    const int size = min(group, pairs - g * group);
+    tile = rest / size;
+    pair = g * group + rest - tile * size;
+  }
+};
+
+inline TileOrder tile_order(int tiles, int pairs, int64_t bytes_per_pair) {
+  const int64_t fit = (64ll << 20) / (bytes_per_pair > 0 ? bytes_per_pair : 1);
+  return TileOrder{tiles, pairs, (int)(fit < 1 ? 1 : fit < pairs ? fit : pairs)};
+}
+
 int make_tmap_bthd(CUtensorMap* map, const void* ptr, int dtype, int B, int T, int heads, int D, const int64_t* stride,
                    uint32_t box_rows);
 int device_sm_count();

@@ -67,14 +67,17 @@ struct KeyWalk {
 template <typename E, int DP>
 __global__ void __launch_bounds__(WinFwd<DP>::kThreads, WinFwd<DP>::kCtas)
     window_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                          const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ WindowParams p) {
+                          const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ WindowParams p,
+                          const __grid_constant__ TileOrder order) {
   using L = WinFwd<DP>;
   constexpr int G = L::G, KT = L::KT, KS = L::KS, VS = L::VS, kQ = L::kQ;
   constexpr uint32_t kFmt = std::is_same<E, __half>::value ? 0 : 1;
   extern __shared__ uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int head = blockIdx.y, b = blockIdx.z, kv = head / p.group;
-  const int unit = gridDim.x - 1 - blockIdx.x;  // longest key ranges first
+  int unit, pair;
+  order.at(blockIdx.x, unit, pair);
+  unit = order.tiles - 1 - unit;  // longest key ranges first
+  const int b = pair / p.H, head = pair - b * p.H, kv = head / p.group;
   const int i0 = unit * kQ * G;                 // first query row of the CTA
   const int length = window_length(p, b);
   const int rows = min(p.Tq, length - p.offset);  // query rows with a token
@@ -400,9 +403,11 @@ static int launch_window_forward(const NoiseWindow* a, const WindowParams& p, cu
       make_tmap_bthd(&tv, a->v, a->dtype, a->B, a->Tk, a->Hk, a->D, a->v_stride, L::KT))
     return kStatusBadArgument;
   if (!opt_in(window_forward_kernel<E, DP>, L::kSmem)) return kStatusLaunchFailed;
-  const dim3 grid((a->Tq + L::kQ * L::G - 1) / (L::kQ * L::G), a->H, a->B);
+  const int64_t units = (a->Tq + L::kQ * L::G - 1) / (L::kQ * L::G), pairs = (int64_t)a->B * a->H;
+  if (units * pairs > INT32_MAX) return kStatusUnsupported;
+  const TileOrder order = tile_order((int)units, (int)pairs, (int64_t)a->Tk * a->D * 4 / p.group);
   LaunchScope scope(kKindAttention, s);
-  window_forward_kernel<E, DP><<<grid, L::kThreads, L::kSmem, s>>>(tq, tk, tv, p);
+  window_forward_kernel<E, DP><<<(unsigned)(units * pairs), L::kThreads, L::kSmem, s>>>(tq, tk, tv, p, order);
   return cudaGetLastError() == cudaSuccess ? kStatusOk : kStatusLaunchFailed;
 }
 

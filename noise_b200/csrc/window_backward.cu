@@ -4,15 +4,15 @@
 //   Delta_i = sum_d dO_id O_id,   dP = dO V^T,   dS = P * (dP - Delta)
 //   dV = P^T dO,   dK = scale dS^T Q,   dQ = scale dS K
 //
-// Three launches (a fourth where a key tile's queries are split):
-//   1. window_stats: Delta, and -lse in base 2, of every query row, in chunks of 64 rows the others load whole.
-//   2. keys' side:    one CTA = 128 keys, streaming the 64-query tiles of every head of the group that see them.
-//   3. queries' side: one CTA = 128 queries of one head, streaming the 64-key tiles they see.
+// Two launches (more where a key tile's queries are split):
+//   window_stats:    Delta, and -lse in base 2, of every query row, in chunks of 64 rows the others load whole.
+//   window_backward: the keys' side, one CTA = 128 keys, streaming the 64-query tiles of every head of the group that
+//                    see them; then the queries' side, one CTA = 128 queries of one head, streaming the 64-key tiles.
 // S and dP are formed on both sides: 7 products a block of pairs instead of 5, but every gradient is summed in
 // one CTA's tensor memory in a fixed order. Adding dQ across key tiles with atomics would save the two products
 // and make the result depend on timing.
 //
-// Sides 2 and 3 are one kernel. X0, X1 are the CTA's own 128-row tiles, Y0, Y1 the streamed 64-row tiles:
+// The sides have one body. X0, X1 are the CTA's own 128-row tiles, Y0, Y1 the streamed 64-row tiles:
 //   S  = X0 Y0^T, dP = X1 Y1^T  (both operands in shared memory, accumulators in tensor memory)
 //   P and dS, as 16-bit pairs over the columns that S and dP lay in, are the A operands of
 //   keys' side (X = K, V; Y = Q, dO; rows are keys):     dV += P Y1, dK += dS Y0
@@ -38,7 +38,13 @@ struct WindowGrad {
   int stat_tiles;
   void *dq, *dk, *dv;  // contiguous [B, T, heads, D]
   float* partial;      // [slot][2][128][D] sums of split key tiles
-  int sink_tiles, sink_splits, splits;  // key tiles that hold sinks come first
+  int sink_tiles, sink_splits, splits, slots;  // key tiles that hold sinks come first; slots per (sequence, key head)
+  TileOrder keys, queries;
+};
+
+// Boxes of 128 rows for a CTA's own tiles, of 64 for the streamed ones.
+struct WindowMaps {
+  CUtensorMap k128, v128, q64, o64, q128, o128, k64, v64;
 };
 
 template <int DP>
@@ -94,20 +100,21 @@ __global__ void __launch_bounds__(256) window_stats_kernel(const __nv_bfloat16* 
   }
 }
 
+// One CTA of either side; `index` is its place in that side's order.
 template <int DP, bool kKeys>
-__global__ void __launch_bounds__(WinBwd<DP>::kThreads, WinBwd<DP>::kCtas)
-    window_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __grid_constant__ CUtensorMap tm_x1,
-                           const __grid_constant__ CUtensorMap tm_y0, const __grid_constant__ CUtensorMap tm_y1,
-                           const __grid_constant__ WindowGrad p) {
+__device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUtensorMap& tm_x1, const CUtensorMap& tm_y0,
+                                            const CUtensorMap& tm_y1, const WindowGrad& p, int index) {
   using L = WinBwd<DP>;
   constexpr int NB = L::NB, YS = L::YS, kX = L::kX, kY = L::kY;
   extern __shared__ uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const WindowParams& w = p.w;
-  const int b = blockIdx.z;
+  const int heads_k = w.H / w.group;
+  int place, pair;  // place: the keys' side's (tile, split), or the query tile from the last
+  (kKeys ? p.keys : p.queries).at(index, place, pair);
+  const int b = pair / (kKeys ? heads_k : w.H), own_head = pair - b * (kKeys ? heads_k : w.H);
   const int length = window_length(w, b);
   const int rows = min(w.Tq, length - w.offset);  // query rows with a token (may be <= 0)
-  const int heads_k = w.H / w.group;
 
   // this CTA's X tile and its items, each one streamed Y tile
   int x0, kv, head0, items, begin = 0, slot = -1;
@@ -115,21 +122,17 @@ __global__ void __launch_bounds__(WinBwd<DP>::kThreads, WinBwd<DP>::kCtas)
   int sink_y = 0;                    // queries' side: sink tiles [0, sink_y), then first_y ..
   if (kKeys) {
     int tile, split, splits;
-    const int sink_ctas = p.sink_tiles * p.sink_splits;
-    if ((int)blockIdx.x < sink_ctas) {
-      tile = blockIdx.x / p.sink_splits, split = blockIdx.x - tile * p.sink_splits, splits = p.sink_splits;
-      if (splits > 1) slot = blockIdx.x;
+    const int sink_places = p.sink_tiles * p.sink_splits;
+    if (place < sink_places) {
+      tile = place / p.sink_splits, split = place - tile * p.sink_splits, splits = p.sink_splits;
+      if (splits > 1) slot = place;
     } else {
-      const int r = blockIdx.x - sink_ctas;
+      const int r = place - sink_places;
       tile = p.sink_tiles + r / p.splits, split = r % p.splits, splits = p.splits;
-      if (splits > 1) slot = (p.sink_splits > 1 ? sink_ctas : 0) + r;
+      if (splits > 1) slot = (p.sink_splits > 1 ? sink_places : 0) + r;
     }
-    if (slot >= 0) {
-      const int slots = (p.sink_splits > 1 ? sink_ctas : 0) +
-                        (p.splits > 1 ? (int)gridDim.x - sink_ctas : 0);
-      slot += (b * heads_k + (int)blockIdx.y) * slots;
-    }
-    x0 = tile * kX, kv = blockIdx.y, head0 = kv * w.group;
+    if (slot >= 0) slot += pair * p.slots;
+    x0 = tile * kX, kv = own_head, head0 = kv * w.group;
     const int last_key = min(x0 + kX, length) - 1;
     const int lo = max(0, x0 - w.offset);
     const int hi = x0 < w.sinks ? rows - 1 : min(rows - 1, last_key + w.window - w.offset);
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(WinBwd<DP>::kThreads, WinBwd<DP>::kCtas)
     begin = min(all, split * share);
     items = min(all, begin + share) - begin;
   } else {
-    x0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * kX, head0 = blockIdx.y, kv = head0 / w.group;
+    x0 = (p.queries.tiles - 1 - place) * kX, head0 = own_head, kv = head0 / w.group;
     first_y = per_head = items = 0;
     if (x0 < rows) {
       const int q_first = w.offset + x0, q_last = min(w.offset + x0 + kX, length) - 1;
@@ -437,6 +440,16 @@ __global__ void __launch_bounds__(WinBwd<DP>::kThreads, WinBwd<DP>::kCtas)
   }
 }
 
+// Both sides in one launch, the keys' side first: its CTAs have the most work.
+template <int DP>
+__global__ void __launch_bounds__(WinBwd<DP>::kThreads, WinBwd<DP>::kCtas)
+    window_backward_kernel(const __grid_constant__ WindowMaps m, const __grid_constant__ WindowGrad p, int key_ctas) {
+  if ((int)blockIdx.x < key_ctas)
+    window_side<DP, true>(m.k128, m.v128, m.q64, m.o64, p, blockIdx.x);
+  else
+    window_side<DP, false>(m.q128, m.o128, m.k64, m.v64, p, blockIdx.x - key_ctas);
+}
+
 // dK and dV of split key tiles: their partial sums added in order. One thread per four columns.
 __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WindowGrad p, int slots, int first_tile,
                                                           int tiles, int splits, int slot0) {
@@ -495,30 +508,31 @@ static WindowPlan window_plan(const NoiseWindow* a) {
 }
 
 template <int DP>
-static int launch_window_backward(const NoiseWindow* a, const void* dout, const int64_t* ds, const WindowGrad& g,
+static int launch_window_backward(const NoiseWindow* a, const void* dout, const int64_t* ds, WindowGrad& g,
                                   const WindowPlan& plan, cudaStream_t s) {
   using L = WinBwd<DP>;
-  static KernelOptIn keys_in, queries_in;
-  if (!keys_in(window_backward_kernel<DP, true>, L::kSmem) || !queries_in(window_backward_kernel<DP, false>, L::kSmem))
-    return kStatusLaunchFailed;
-  CUtensorMap k128, v128, q64, o64, q128, o128, k64, v64;
-  auto map = [&](CUtensorMap* m, const void* ptr, int T, int heads, const int64_t* stride, int box) {
-    return make_tmap_bthd(m, ptr, NOISE_BF16, a->B, T, heads, a->D, stride, (uint32_t)box);
+  static KernelOptIn opt_in;
+  if (!opt_in(window_backward_kernel<DP>, L::kSmem)) return kStatusLaunchFailed;
+  WindowMaps m;
+  auto map = [&](CUtensorMap* t, const void* ptr, int T, int heads, const int64_t* stride, int box) {
+    return make_tmap_bthd(t, ptr, NOISE_BF16, a->B, T, heads, a->D, stride, (uint32_t)box);
   };
-  if (map(&k128, a->k, a->Tk, a->Hk, a->k_stride, L::kX) || map(&v128, a->v, a->Tk, a->Hk, a->v_stride, L::kX) ||
-      map(&q64, a->q, a->Tq, a->H, a->q_stride, L::kY) || map(&o64, dout, a->Tq, a->H, ds, L::kY) ||
-      map(&q128, a->q, a->Tq, a->H, a->q_stride, L::kX) || map(&o128, dout, a->Tq, a->H, ds, L::kX) ||
-      map(&k64, a->k, a->Tk, a->Hk, a->k_stride, L::kY) || map(&v64, a->v, a->Tk, a->Hk, a->v_stride, L::kY))
+  if (map(&m.k128, a->k, a->Tk, a->Hk, a->k_stride, L::kX) || map(&m.v128, a->v, a->Tk, a->Hk, a->v_stride, L::kX) ||
+      map(&m.q64, a->q, a->Tq, a->H, a->q_stride, L::kY) || map(&m.o64, dout, a->Tq, a->H, ds, L::kY) ||
+      map(&m.q128, a->q, a->Tq, a->H, a->q_stride, L::kX) || map(&m.o128, dout, a->Tq, a->H, ds, L::kX) ||
+      map(&m.k64, a->k, a->Tk, a->Hk, a->k_stride, L::kY) || map(&m.v64, a->v, a->Tk, a->Hk, a->v_stride, L::kY))
     return kStatusBadArgument;
   const int plain = plan.k_tiles - plan.sink_tiles;
-  LaunchScope scope(kKindAttention, s, 3 + (plan.sink_splits > 1) + (plan.splits > 1));
+  const int64_t group = a->H / a->Hk, places = plan.sink_tiles * plan.sink_splits + (int64_t)plain * plan.splits;
+  const int64_t key_ctas = places * a->B * a->Hk, query_ctas = (int64_t)((a->Tq + 127) / 128) * a->B * a->H;
+  if (key_ctas + query_ctas > INT32_MAX) return kStatusUnsupported;
+  g.keys = tile_order((int)places, a->B * a->Hk, (int64_t)a->Tq * a->D * 4 * group);
+  g.queries = tile_order((a->Tq + 127) / 128, a->B * a->H, (int64_t)a->Tk * a->D * 4 / group);
+  LaunchScope scope(kKindAttention, s, 2 + (plan.sink_splits > 1) + (plan.splits > 1));
   window_stats_kernel<<<dim3(plan.q_tiles, a->H, a->B), 256, 0, s>>>(
       reinterpret_cast<const __nv_bfloat16*>(a->out), reinterpret_cast<const __nv_bfloat16*>(dout), a->B > 1 ? ds[0] : 0,
       a->Tq > 1 ? ds[1] : 0, a->H > 1 ? ds[2] : 0, g.w, const_cast<float*>(g.stat));
-  window_backward_kernel<DP, true><<<dim3(plan.sink_tiles * plan.sink_splits + plain * plan.splits, a->Hk, a->B),
-                                     L::kThreads, L::kSmem, s>>>(k128, v128, q64, o64, g);
-  window_backward_kernel<DP, false>
-      <<<dim3((a->Tq + 127) / 128, a->H, a->B), L::kThreads, L::kSmem, s>>>(q128, o128, k64, v64, g);
+  window_backward_kernel<DP><<<(unsigned)(key_ctas + query_ctas), L::kThreads, L::kSmem, s>>>(m, g, (int)key_ctas);
   const int join = 64;
   if (plan.sink_splits > 1)
     window_join_kernel<<<dim3(min(join, plan.sink_tiles * a->D / 4), a->Hk, a->B), 256, 0, s>>>(
@@ -558,7 +572,7 @@ extern "C" int noise_window_attention_backward(const NoiseWindow* a, const void*
   g.stat = reinterpret_cast<const float*>(workspace), g.stat_tiles = plan.q_tiles;
   g.partial = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + plan.stat_bytes);
   g.dq = dq, g.dk = dk, g.dv = dv;
-  g.sink_tiles = plan.sink_tiles, g.sink_splits = plan.sink_splits, g.splits = plan.splits;
+  g.sink_tiles = plan.sink_tiles, g.sink_splits = plan.sink_splits, g.splits = plan.splits, g.slots = plan.slots;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return a->D <= 64 ? launch_window_backward<64>(a, dout, dout_stride, g, plan, s)
                     : launch_window_backward<128>(a, dout, dout_stride, g, plan, s);
