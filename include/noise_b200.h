@@ -370,7 +370,7 @@ int noise_window_token(const NoiseWindow* args, void* stream);
  * s = softcap tanh(z / softcap) / temperature (softcap 0: z / temperature), p = softmax of a row's teacher
  * logits / temperature, loss = temperature^2 sum_k p_k (log p_k - s[id_k] + logsumexp(s)). Entries whose id is
  * outside [0, V) are absent; equal ids add up; a row without an entry above -inf has loss and gradient 0.
- * lse_in null: loss [N] (and lse [N], optional: logsumexp(s)) are written, and, with grad, the gradient of
+ * lse_in null: loss [N] (and lse [N] in 64 bits, optional: logsumexp(s)) are written, and, with grad, the gradient of
  * sum_n dloss[n] loss[n] (dloss null: of sum_n loss[n]) in the same pass, for
  * V <= noise_distill_max_vocab(dtype, softcap > 0). lse_in given (the lse of an earlier call): only grad.
  * grad [N, V] of `dtype`, row stride grad_ld; it must not overlap logits. */
@@ -379,8 +379,10 @@ typedef struct NoiseDistill {
   float temperature, softcap;
   int64_t N, ld, ids_ld, teacher_ld, grad_ld;
   const void *logits, *ids, *teacher;
-  const float *dloss, *lse_in;
-  float *loss, *lse;
+  const float* dloss;
+  const double* lse_in;
+  float* loss;
+  double* lse;
   void* grad;
 } NoiseDistill;
 int64_t noise_distill_max_vocab(int dtype, int softcap);

@@ -7,11 +7,20 @@
 //   d loss / dz_j = tau (exp(s_j - lse) - sum over k with id_k = j of p_k) (1 - tanh^2(z_j / c))
 // An entry whose id is outside [0, V) is absent; a row without an entry above -inf has loss and gradient 0.
 //
-// Bound: HBM. The loss reads a row once, with a running maximum and sum in each thread. Loss and gradient
-// together read it once and write it once: the row's values stay in shared memory between the two
-// halves of the work, s as fp32 where the soft cap made it costly, the loaded words otherwise. A row
-// too long for one CTA, or one of a few rows, is spread over a cluster of up to 8 CTAs whose maxima and
-// sums meet through distributed shared memory, so no second launch or workspace is needed.
+// Bound: HBM, with the special-function unit (16 results a cycle and SM) next: a soft-capped logit takes three
+// (the exponential and reciprocal of its tanh, the exponential of s). The loss reads a row once. Loss and gradient
+// together read it once and write it once; the row waits between the two halves in shared memory:
+//   - with a soft cap s <= c / tau, so that is the sums' reference, no maximum is sought, and what waits is
+//     exp(s - c / tau) (1 - tanh^2), which the second half only multiplies by one factor of the row;
+//   - without one a thread takes the maximum of its first values as its reference and looks for another only
+//     when a sum leaves fp32's safe range; what waits are the loaded words, and their exponential is taken again.
+// What it takes is bytes in flight: a CTA is 128 threads, eight to an SM, and each thread copies its own 16-byte
+// slots into shared memory six batches ahead (with loads to registers, 137 instead of 111 us for 16,384 rows of 4,096
+// soft-capped fp32 logits with 32 entries, loss and gradient; CTAs of 256 threads 180). That is 4.9 TB/s; 2,047 rows of
+// 50,257 bf16 logits take 131 us for the loss and then the gradient from its lse, 4.7 TB/s.
+//
+// A row too long for one CTA, or one of a few rows, is spread over a cluster of up to 8 CTAs whose sums meet
+// through distributed shared memory, so no second launch or workspace is needed.
 //
 // The K entries are handled apart from the dense pass: every column is first written as if no entry
 // named it, then the thread of an id's first entry rewrites that column with the sum over the entries
@@ -22,12 +31,18 @@
 
 namespace noise {
 
-constexpr int kDsThreads = 256, kDsWarps = kDsThreads / 32;
+constexpr int kDsThreads = 128, kDsWarps = kDsThreads / 32;
+constexpr int kDsResident = 8;           // CTAs an SM holds
 constexpr int kDsMaxK = 1024;
 constexpr int kDsMaxCluster = 8;
 constexpr int kDsRowBytes = 192 * 1024;  // shared memory that holds a CTA's part of a row, at most
+constexpr int kDsBatch = 2, kDsAhead = 6;  // slots of a batch; batches a thread has in flight
+constexpr int kDsRing = kDsAhead * kDsBatch * kDsThreads * 16;
 
 enum : int { kDsLoss = 0, kDsGrad = 1, kDsBoth = 2 };
+// No soft cap; one whose c / tau bounds every exponential within fp32 (2 c / tau <= 80); any other.
+enum : int { kCapNone = 0, kCapBound = 1, kCapFree = 2 };
+constexpr float kDsBoundCap = 40.f;
 
 struct DistillParams {
   const void* logits;
@@ -38,14 +53,14 @@ struct DistillParams {
   const void* teacher;
   int64_t teacher_ld;
   int teacher_type;
-  const float* up;      // gradient of each row's loss (null: 1)
-  const float* lse_in;  // gradient from a saved lse
+  const float* up;       // gradient of each row's loss (null: 1)
+  const double* lse_in;  // gradient from a saved lse
   float* loss;
-  float* lse;
+  double* lse;
   void* grad;
   int64_t grad_ld;
   int64_t rows;
-  int V, K, parts;      // parts: CTAs per row
+  int V, K, parts;       // parts: CTAs per row
   float tau, cap;
 };
 
@@ -57,50 +72,66 @@ struct DsSlot {
 };
 
 template <typename E>
-__device__ __forceinline__ void slot_values(const uint4& w, float (&v)[DsSlot<E>::kN]) {
+__device__ __forceinline__ void slot_values(const uint4& w, float2 (&v)[DsSlot<E>::kN / 2]) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
   if constexpr (sizeof(E) == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(u[i]);
+    v[0] = make_float2(__uint_as_float(u[0]), __uint_as_float(u[1]));
+    v[1] = make_float2(__uint_as_float(u[2]), __uint_as_float(u[3]));
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack2<E>(u[i]);
-      v[2 * i] = f.x, v[2 * i + 1] = f.y;
-    }
+    for (int i = 0; i < 4; ++i) v[i] = unpack2<E>(u[i]);
   }
 }
 
 template <typename E>
-__device__ __forceinline__ uint4 slot_pack(const float (&v)[DsSlot<E>::kN]) {
+__device__ __forceinline__ uint4 slot_pack(const float2 (&v)[DsSlot<E>::kN / 2]) {
   if constexpr (sizeof(E) == 4)
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
   else
-    return make_uint4(pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3]), pack2<E>(v[4], v[5]), pack2<E>(v[6], v[7]));
+    return make_uint4(pack2<E>(v[0].x, v[0].y), pack2<E>(v[1].x, v[1].y), pack2<E>(v[2].x, v[2].y),
+                      pack2<E>(v[3].x, v[3].y));
 }
 
-// exp of a difference that is <= 0 up to rounding.
-__device__ __forceinline__ float ds_exp(float x) { return expf(x); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 ex2_pair(float2 x) { return make_float2(ex2_approx(x.x), ex2_approx(x.y)); }
 
-// A running maximum m and the sum of exp(. - m); an empty or all -inf set is (-inf, 0).
+// tanh to about 2 ulp. Away from 0 from e = exp(-2 |x|): (1 - e) / (1 + e). Near 0, where 1 - e would cancel, from a
+// polynomial x + x^3 Q(x^2), |x| <= 0.55: Q is a least-squares fit of degree 4 at Chebyshev nodes, off by 4e-9 of tanh.
+__device__ __forceinline__ float ds_tanh(float x) {
+  const float a = fabsf(x), u = x * x;
+  const float e = ex2_approx(a * -2.8853900817779268f);
+  const float far = (1.f - e) * rcp_approx(1.f + e);
+  float q = fmaf(-0.006615746766f, u, 0.0213127397f);
+  q = fmaf(q, u, -0.05391006544f);
+  q = fmaf(q, u, 0.1333311796f);
+  q = fmaf(q, u, -0.3333333135f);
+  const float near = fmaf(x * u, q, x);
+  return a < 0.55f ? near : copysignf(far, x);
+}
+__device__ __forceinline__ float2 ds_tanh(float2 x) { return make_float2(ds_tanh(x.x), ds_tanh(x.y)); }
+
+// A reference m and the sum of 2^(scale (. - m)); an empty or all -inf set is (-inf, 0). The difference is taken
+// before the scale, so that values near the type's lowest do not turn into -inf.
 struct MaxSum {
   float m, s;
-  __device__ __forceinline__ void join(float om, float os) {
+  __device__ __forceinline__ void join(float om, float os, float scale = 1.f) {
     const float top = fmaxf(m, om);
     const float base = top == -INFINITY ? 0.f : top;
-    s = (m == -INFINITY ? s : s * ds_exp(m - base)) + (om == -INFINITY ? os : os * ds_exp(om - base));
+    s = (m == -INFINITY ? s : s * exp2f((m - base) * scale)) + (om == -INFINITY ? os : os * exp2f((om - base) * scale));
     m = top;
   }
 };
 
-template <typename E, int kMode, bool kCap>
-__global__ void __launch_bounds__(kDsThreads) distill_kernel(const __grid_constant__ DistillParams p) {
+template <typename E, int kMode, int kCap>
+__global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const __grid_constant__ DistillParams p) {
   constexpr int N = DsSlot<E>::kN;
   constexpr bool kHold = kMode == kDsBoth;  // the row stays in shared memory
-  extern __shared__ uint4 hold[];           // raw slots, or with a soft cap N / 4 planes of s
-  __shared__ int s_id[kDsMaxK];
-  __shared__ float s_p[kDsMaxK];
-  __shared__ float red[2][kDsWarps];
+  constexpr bool kBound = kCap == kCapBound;
+  constexpr float kLog2e = 1.4426950408889634f;
+  // the row's slots (kHold; with a bound soft cap N / 4 planes of fp32 per slot), or a ring of batches in flight
+  extern __shared__ uint4 hold[];
+  __shared__ __align__(16) int s_id[kDsMaxK];
+  __shared__ float red[5][kDsWarps];
   __shared__ float2 part;  // this CTA's (m, s), read by the cluster
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.x / p.parts;
@@ -112,120 +143,167 @@ __global__ void __launch_bounds__(kDsThreads) distill_kernel(const __grid_consta
   const int share = (slots + p.parts - 1) / p.parts;
   const int begin = min(slots, rank * share), end = min(slots, begin + share);
   const float inv_tau = 1.0f / p.tau, inv_cap = kCap ? 1.0f / p.cap : 0.f;
-  const float s_of = kCap ? p.cap * inv_tau : inv_tau;  // s = s_of * tanh(z / c), or s_of * z
+  // s in base 2 is scale * v, with v = z, or tanh(z / c)
+  const float scale = (kCap ? p.cap : 1.f) * inv_tau * kLog2e;
 
-  auto load = [&](int slot) {
-    if (slot * N >= phase && (slot + 1) * N <= p.V + phase)
-      return __ldcs(reinterpret_cast<const uint4*>(z0) + slot);
-    float v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = slot * N + i - phase;
-      v[i] = e >= 0 && e < p.V ? to_f32(z[e]) : -INFINITY;
-    }
-    return slot_pack<E>(v);
+  // This CTA's whole slots, and its share of the row's at most two partial ones: one element after the other, by
+  // the first thread.
+  const int head = (N - phase) % N, tail = head + (p.V - head > 0 ? (p.V - head) / N * N : 0);  // [head, tail): whole slots
+  const int skip = phase ? 1 : 0;
+  const int first = max(begin, skip), last = min(end, skip + (tail - head) / N);
+  const bool has_head = phase && begin == 0 && end > 0, has_tail = tail < p.V && end == slots && end > begin;
+  auto edges = [&](auto&& f) {
+    if (tid != 0) return;
+    if (has_head)
+      for (int e = 0; e < min(head, p.V); ++e) f(e);
+    if (has_tail)
+      for (int e = max(tail, head); e < p.V; ++e) f(e);
   };
-  auto to_s = [&](float x) { return kCap ? s_of * tanhf(x * inv_cap) : s_of * x; };
+  const uint4* z16 = reinterpret_cast<const uint4*>(z0);
+  // f(batch of slots, its first slot, how many) for this thread's slots first + tid, + kDsThreads, ..: each thread
+  // copies its own slots into its own places, kDsAhead batches ahead
+  auto place = [&](int batch, int u, int slot) {
+    return kHold ? slot - begin : ((batch % kDsAhead) * kDsBatch + u) * kDsThreads + tid;
+  };
+  auto issue = [&](int batch) {
+#pragma unroll
+    for (int u = 0; u < kDsBatch; ++u) {
+      const int slot = first + tid + (batch * kDsBatch + u) * kDsThreads;
+      if (slot < last) cp_async16(smem_u32(hold + place(batch, u, slot)), z16 + slot);
+    }
+    cp_async_commit();
+  };
+  auto start = [&] {
+#pragma unroll
+    for (int i = 0; i < kDsAhead - 1; ++i) issue(i);
+  };
+  auto sweep = [&](auto&& f) {
+    int batch = 0;
+    for (int slot = first + tid; slot < last; slot += kDsBatch * kDsThreads, ++batch) {
+      issue(batch + kDsAhead - 1);
+      cp_async_wait<kDsAhead - 1>();
+      uint4 w[kDsBatch];
+#pragma unroll
+      for (int u = 0; u < kDsBatch; ++u)
+        if (slot + u * kDsThreads < last) w[u] = hold[place(batch, u, slot + u * kDsThreads)];
+      f(w, slot, min(kDsBatch, (last - slot + kDsThreads - 1) / kDsThreads));
+    }
+  };
+  start();
+  auto value = [&](float2 x) { return kCap ? ds_tanh(__fmul2_rn(x, both(inv_cap))) : x; };
+  auto value1 = [&](float x) { return kCap ? ds_tanh(x * inv_cap) : x; };
 
-  // the teacher's entries: p_k = exp((t_k - max) / tau) / mass, 0 for absent ones. The maximum is taken off
-  // before the division, so that entries at the type's lowest value do not turn into -inf.
-  float top = -INFINITY;
-  for (int k = tid; k < p.K; k += kDsThreads) {
-    const int64_t at = row * p.ids_ld + k;
-    const int64_t id = p.ids64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + at)
-                               : (int64_t)__ldg(reinterpret_cast<const int*>(p.ids) + at);
-    const int64_t tt = row * p.teacher_ld + k;
-    float t = p.teacher_type == NOISE_FP32   ? reinterpret_cast<const float*>(p.teacher)[tt]
-              : p.teacher_type == NOISE_BF16 ? to_f32(reinterpret_cast<const __nv_bfloat16*>(p.teacher)[tt])
-                                             : to_f32(reinterpret_cast<const __half*>(p.teacher)[tt]);
-    const bool have = id >= 0 && id < p.V;
-    t = have ? t : -INFINITY;
-    s_id[k] = have ? (int)id : -1;
-    s_p[k] = t;
-    top = t != t ? t : fmaxf(top, t);
-  }
-  // NaN must survive the maximum: it is carried as the sum instead
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) red[0][warp] = top;
-  __syncthreads();
-  top = red[0][0];
-#pragma unroll
-  for (int w = 1; w < kDsWarps; ++w) top = fmaxf(top, red[0][w]);
-  float mass = 0.f;
-  for (int k = tid; k < p.K; k += kDsThreads) {
-    if (top == -INFINITY) mass += s_p[k] == -INFINITY ? 0.f : s_p[k];  // no entry, or NaN
-    else mass += ds_exp((s_p[k] - top) * inv_tau);
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
-  if (lane == 0) red[1][warp] = mass;
-  __syncthreads();
-  mass = red[1][0];
-#pragma unroll
-  for (int w = 1; w < kDsWarps; ++w) mass += red[1][w];
-  const bool empty = mass == 0.f;
-  const float log_mass = logf(mass), inv_mass = 1.0f / mass;
+  // Entry k: its id (-1: absent) and logit. A thread keeps its first one, k = tid, in registers from the start.
+  auto entry = [&](int k, int& id) {
+    const int64_t at = row * p.ids_ld + k, tt = row * p.teacher_ld + k;
+    const int64_t i = p.ids64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + at)
+                              : (int64_t)__ldg(reinterpret_cast<const int*>(p.ids) + at);
+    const float t = p.teacher_type == NOISE_FP32   ? reinterpret_cast<const float*>(p.teacher)[tt]
+                    : p.teacher_type == NOISE_BF16 ? to_f32(reinterpret_cast<const __nv_bfloat16*>(p.teacher)[tt])
+                                                   : to_f32(reinterpret_cast<const __half*>(p.teacher)[tt]);
+    const bool have = i >= 0 && i < p.V;
+    id = have ? (int)i : -1;
+    return have ? t : -INFINITY;
+  };
+  int id0 = -1;
+  float t0 = -INFINITY;
+  if (tid < p.K) t0 = entry(tid, id0);
 
-  float lse = 0.f;
+  MaxSum a{kBound ? scale : -INFINITY, 0.f};
   if constexpr (kMode != kDsGrad) {
-    MaxSum a{-INFINITY, 0.f};
-    for (int s0 = begin + tid; s0 < end; s0 += 4 * kDsThreads) {
-      uint4 w[4];
+    // one slot's sum under the reference as it stands
+    auto add = [&](const uint4& w, int slot, float2& sum) {
+      float2 v[N / 2];
+      slot_values<E>(w, v);
+      if constexpr (kBound) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (s0 + u * kDsThreads < end) w[u] = load(s0 + u * kDsThreads);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int slot = s0 + u * kDsThreads;
-        if (slot >= end) break;
-        float v[N];
-        slot_values<E>(w[u], v);
-        const bool edge = slot * N < phase || (slot + 1) * N > p.V + phase;
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = to_s(v[i]);
-        if (kCap && edge) {  // tanh turned the places outside the row into -c
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const int e = slot * N + i - phase;
-            if (e < 0 || e >= p.V) v[i] = -INFINITY;
-          }
+        for (int i = 0; i < N / 2; ++i) {
+          const float2 th = value(v[i]);
+          const float2 e = ex2_pair(__ffma2_rn(th, both(scale), both(-scale)));
+          sum = __fadd2_rn(sum, e);
+          if (kHold) v[i] = __fmul2_rn(e, __ffma2_rn(make_float2(-th.x, -th.y), th, both(1.f)));
         }
         if constexpr (kHold) {
-          if constexpr (kCap) {
 #pragma unroll
-            for (int i = 0; i < N / 4; ++i)
-              reinterpret_cast<float4*>(hold)[i * share + slot - begin] =
-                  make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-          } else {
-            hold[slot - begin] = w[u];
-          }
+          for (int i = 0; i < N / 4; ++i)
+            reinterpret_cast<float4*>(hold)[i * share + slot - begin] =
+                make_float4(v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y);
         }
-        float m = v[0];
+      } else {
+        const float2 off = both(a.m == -INFINITY ? 0.f : -a.m);
 #pragma unroll
-        for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
-        if (m > a.m) {
-          a.s = a.m == -INFINITY ? a.s : a.s * ds_exp(a.m - m);
-          a.m = m;
-        }
-        const float base = a.m == -INFINITY ? 0.f : a.m;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum += ds_exp(v[i] - base);
-        a.s += sum;
+        for (int i = 0; i < N / 2; ++i) sum = __fadd2_rn(sum, ex2_pair(__ffma2_rn(value(v[i]), both(scale), off)));
       }
-    }
+    };
+    // a reference that the slots from `slot` on, `count` of them, do not overflow
+    auto raise = [&](int slot, int count) {
+      float m = -INFINITY;
+#pragma unroll 1
+      for (int e = slot * N - phase; count; e += kDsThreads * N, --count)
+#pragma unroll 1
+        for (int i = 0; i < N; ++i) m = fmaxf(m, scale * value1(to_f32(z[e + i])));
+      if (m > a.m) a.s = a.m == -INFINITY ? a.s : a.s * exp2f(a.m - m), a.m = m;
+    };
+    auto take = [&](const uint4* w, int slot, int count) {
+      if (!kBound && a.m == -INFINITY) raise(slot, count);
+      float2 sum = both(0.f);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float om = __shfl_xor_sync(0xffffffffu, a.m, o), os = __shfl_xor_sync(0xffffffffu, a.s, o);
-      a.join(om, os);
+      for (int u = 0; u < kDsBatch; ++u)
+        if (u < count) add(w[u], slot + u * kDsThreads, sum);
+      if (!kBound && !(sum.x + sum.y < 1e30f)) {
+        raise(slot, count);
+        sum = both(0.f);
+#pragma unroll
+        for (int u = 0; u < kDsBatch; ++u)
+          if (u < count) add(w[u], slot + u * kDsThreads, sum);
+      }
+      a.s += sum.x + sum.y;
+    };
+    sweep(take);
+    edges([&](int e) {
+      const float x = value1(to_f32(z[e])) * scale;
+      if (kBound) a.s += ex2_approx(x - scale);
+      else a.join(x, x == -INFINITY ? 0.f : 1.f);
+    });
+  }
+  // the teacher's maximum and mass: p_k = 2^(t_scale (t_k - max)) / mass, 0 for absent entries
+  const float t_scale = inv_tau * kLog2e;
+  MaxSum c{t0, t0 == -INFINITY ? 0.f : 1.f};
+  if (tid < p.K) s_id[tid] = id0;
+  for (int k = tid + kDsThreads; k < p.K; k += kDsThreads) {
+    int id;
+    const float t = entry(k, id);
+    s_id[k] = id;
+    c.join(t, t == -INFINITY ? 0.f : 1.f, t_scale);
+  }
+  const float z_id = id0 >= 0 ? to_f32(z[id0]) : 0.f;
+
+  // one sweep for the row's sum and the teacher's
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    if (kMode != kDsGrad) {
+      const float os = __shfl_xor_sync(0xffffffffu, a.s, o);
+      if (kBound) a.s += os;
+      else a.join(__shfl_xor_sync(0xffffffffu, a.m, o), os);
     }
-    __syncthreads();  // red's earlier readers are done
-    if (lane == 0) red[0][warp] = a.m, red[1][warp] = a.s;
-    __syncthreads();
+    if (warp * 32 < p.K) c.join(__shfl_xor_sync(0xffffffffu, c.m, o), __shfl_xor_sync(0xffffffffu, c.s, o), t_scale);
+  }
+  if (lane == 0) red[0][warp] = a.m, red[1][warp] = a.s, red[2][warp] = c.m, red[3][warp] = c.s;
+  __syncthreads();
+  c = MaxSum{red[2][0], red[3][0]};
+#pragma unroll
+  for (int w = 1; w < kDsWarps; ++w)
+    if (w * 32 < p.K) c.join(red[2][w], red[3][w], t_scale);
+  const float top = c.m, mass = c.s;
+  const bool empty = mass == 0.f;
+  const float inv_mass = 1.0f / mass;
+  if constexpr (kMode != kDsGrad) {
     a = MaxSum{red[0][0], red[1][0]};
 #pragma unroll
-    for (int w = 1; w < kDsWarps; ++w) a.join(red[0][w], red[1][w]);
+    for (int w = 1; w < kDsWarps; ++w) {
+      if (kBound) a.s += red[1][w];
+      else a.join(red[0][w], red[1][w]);
+    }
     if (p.parts > 1) {
       if (tid == 0) part = make_float2(a.m, a.s);
       cluster_sync();
@@ -237,122 +315,165 @@ __global__ void __launch_bounds__(kDsThreads) distill_kernel(const __grid_consta
       a = all;
       cluster_sync();  // no CTA of the cluster leaves while another reads its part
     }
-    lse = a.m == -INFINITY ? logf(a.s) : a.m + logf(a.s);
-  } else {
-    lse = __ldg(p.lse_in + row);
   }
 
+  // the loss's terms, added up behind the dense gradient
   if (kMode != kDsGrad && rank == 0) {
+    const float log_mass = logf(mass), log_sum = log2f(a.s);
     float l = 0.f;
-    for (int k = tid; k < p.K; k += kDsThreads) {
-      if (s_id[k] < 0) continue;
-      const float t = (s_p[k] - top) * inv_tau, pk = ds_exp(t) * inv_mass;
-      if (pk != 0.f) l += pk * ((t - log_mass) + (lse - to_s(to_f32(z[s_id[k]]))));
+    auto term = [&](int id, float t, float x) {
+      const float d = (t - top) * inv_tau, pk = exp2f((t - top) * t_scale) * inv_mass;
+      // lse - s in base 2, from the difference of the reference and s
+      if (id >= 0 && pk != 0.f)
+        l += pk * ((d - log_mass) + 0.6931471805599453f * (log_sum - fmaf(value1(x), scale, -a.m)));
+    };
+    if (tid < p.K) term(id0, t0, z_id);
+    for (int k = tid + kDsThreads; k < p.K; k += kDsThreads) {
+      int id;
+      const float t = entry(k, id);
+      if (id >= 0) term(id, t, to_f32(z[id]));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    __syncthreads();
-    if (lane == 0) red[0][warp] = l;
-    __syncthreads();
-    if (tid == 0) {
-      l = red[0][0];
-#pragma unroll
-      for (int w = 1; w < kDsWarps; ++w) l += red[0][w];
-      p.loss[row] = empty ? 0.f : p.tau * p.tau * l;
-      if (p.lse) p.lse[row] = lse;
-    }
+    if (lane == 0) red[4][warp] = l;
   }
+  auto finish = [&] {  // after a barrier
+    if (kMode == kDsGrad || rank != 0 || tid != 0) return;
+    float l = red[4][0];
+#pragma unroll
+    for (int w = 1; w < kDsWarps; ++w) l += red[4][w];
+    p.loss[row] = empty ? 0.f : p.tau * p.tau * l;
+    // in 64 bits: the gradient's exponentials have the error of this number in common
+    if (p.lse) p.lse[row] = 0.6931471805599453094 * ((double)a.m + log2((double)a.s));
+  };
 
   if constexpr (kMode != kDsLoss) {
     E* g = reinterpret_cast<E*>(p.grad) + row * p.grad_ld;
     const bool same = (int)((reinterpret_cast<uintptr_t>(g) & 15) / sizeof(E)) == phase;
-    const float up = p.tau * (p.up ? __ldg(p.up + row) : 1.0f);
-    const float th_of = kCap ? p.tau * inv_cap : 0.f;  // tanh(z / c) = s tau / c
-    // gradient at a column whose entries hold the mass pj
-    auto value = [&](float s, float pj) {
-      float v = up * (ds_exp(s - lse) - pj);
-      if (kCap) {
-        const float th = s * th_of;
-        v *= fmaf(-th, th, 1.0f);
-      }
-      return empty ? 0.f : v;
+    const float up = empty ? 0.f : p.tau * (p.up ? __ldg(p.up + row) : 1.0f);
+    // softmax(s) is 2^(scale v - ref - low) * factor
+    float ref = a.m, low = 0.f, factor = 1.f / a.s;
+    if constexpr (kMode == kDsGrad) {
+      const double lse2 = p.lse_in[row] * 1.4426950408889634074;
+      ref = (float)lse2, low = (float)(lse2 - (double)ref), factor = 1.f;
+      if (!isfinite(ref)) low = 0.f;
+    }
+    // gradient at a column from v, with the entries' mass pj there
+    auto slope = [&](float v, float pj) {
+      const float d = up * fmaf(ex2_approx(fmaf(v, scale, -ref) - low), factor, -pj);
+      return kCap ? d * fmaf(-v, v, 1.0f) : d;
     };
-    for (int slot = begin + tid; slot < end; slot += kDsThreads) {
-      float v[N];
-      if constexpr (kHold && kCap) {
+    uint4* g16 = reinterpret_cast<uint4*>(g - phase);
+    auto write = [&](int slot, const float2 (&v)[N / 2]) {
+      if (same) {
+        __stcs(g16 + slot, slot_pack<E>(v));
+      } else {
+        E* at = g + slot * N - phase;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) at[2 * i] = from_f32<E>(v[i].x), at[2 * i + 1] = from_f32<E>(v[i].y);
+      }
+    };
+    if (empty) {
+      float2 v[N / 2];
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) v[i] = both(0.f);
+      for (int slot = first + tid; slot < last; slot += kDsThreads) write(slot, v);
+      edges([&](int e) { g[e] = from_f32<E>(0.f); });
+      __syncthreads();
+      finish();
+      return;
+    }
+    const float2 gain = both(up * factor);
+    auto spread = [&](const uint4& w, int slot) {
+      float2 v[N / 2];
+      if constexpr (kHold && kBound) {
 #pragma unroll
         for (int i = 0; i < N / 4; ++i) {
-          const float4 f = reinterpret_cast<const float4*>(hold)[i * share + slot - begin];
-          v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+          const float4 x = reinterpret_cast<const float4*>(hold)[i * share + slot - begin];
+          v[2 * i] = __fmul2_rn(make_float2(x.x, x.y), gain), v[2 * i + 1] = __fmul2_rn(make_float2(x.z, x.w), gain);
         }
       } else {
-        slot_values<E>(kHold ? hold[slot - begin] : load(slot), v);
+        slot_values<E>(w, v);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = to_s(v[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = value(v[i], 0.f);
-      if (same && slot * N >= phase && (slot + 1) * N <= p.V + phase) {
-        __stcs(reinterpret_cast<uint4*>(g - phase) + slot, slot_pack<E>(v));
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int e = slot * N + i - phase;
-          if (e >= 0 && e < p.V) g[e] = from_f32<E>(v[i]);
+        for (int i = 0; i < N / 2; ++i) {
+          const float2 x = value(v[i]);
+          float2 y = __ffma2_rn(x, both(scale), both(-ref));
+          if (kMode == kDsGrad) y = __fadd2_rn(y, both(-low));
+          v[i] = __fmul2_rn(ex2_pair(y), gain);
+          if (kCap) v[i] = __fmul2_rn(v[i], __ffma2_rn(make_float2(-x.x, -x.y), x, both(1.f)));
         }
       }
+      write(slot, v);
+    };
+    if constexpr (kMode == kDsGrad) {
+      sweep([&](const uint4* w, int slot, int count) {
+#pragma unroll
+        for (int u = 0; u < kDsBatch; ++u)
+          if (u < count) spread(w[u], slot + u * kDsThreads);
+      });
+    } else {
+#pragma unroll 4
+      for (int slot = first + tid; slot < last; slot += kDsThreads)
+        spread(kBound ? make_uint4(0u, 0u, 0u, 0u) : hold[slot - begin], slot);
     }
-    if (empty) return;
+    edges([&](int e) { g[e] = from_f32<E>(slope(value1(to_f32(z[e])), 0.f)); });
     __syncthreads();  // the dense stores of this CTA come before its entries' stores
+    finish();
     const int e0 = begin * N - phase, e1 = min(p.V, end * N - phase);
-    for (int k = tid; k < p.K; k += kDsThreads) {
-      const int id = s_id[k];
-      if (id < 0 || id < e0 || id >= e1) continue;
-      bool first = true, again = false;
+    for (int k = tid; k - lane < p.K; k += kDsThreads) {  // whole warps: equal ids among 32 entries by a vote
+      const int id = k < p.K ? s_id[k] : -1;
+      const uint32_t equal = __match_any_sync(0xffffffffu, id);
+      if (id < e0 || id >= e1 || id < 0) continue;
+      bool first = (equal & ((1u << lane) - 1u)) == 0, again = (equal >> lane) > 1u;
+#pragma unroll 8
       for (int i = 0; i < p.K; ++i) {
-        if (s_id[i] != id || i == k) continue;
-        if (i < k) first = false;
-        else again = true;
+        if (p.K <= 32) break;
+        first = first && !(s_id[i] == id && i < k);
+        again = again || (s_id[i] == id && i > k);
       }
       if (!first) continue;
-      float pj = ds_exp((s_p[k] - top) * inv_tau) * inv_mass;
+      int other;
+      float pj = exp2f(((k == tid ? t0 : entry(k, other)) - top) * t_scale) * inv_mass;
       if (again)
         for (int i = k + 1; i < p.K; ++i)
-          if (s_id[i] == id) pj += ds_exp((s_p[i] - top) * inv_tau) * inv_mass;
-      g[id] = from_f32<E>(value(to_s(to_f32(z[id])), pj));
+          if (s_id[i] == id) pj += exp2f((entry(i, other) - top) * t_scale) * inv_mass;
+      g[id] = from_f32<E>(slope(value1(k == tid ? z_id : to_f32(z[id])), pj));
     }
+  } else {
+    __syncthreads();
+    finish();
   }
 }
 
 int device_sm_count();
 
 // Bytes of shared memory that `parts` CTAs each need to hold their part of a row.
-static int64_t ds_hold_bytes(int V, int elem, bool cap, int parts) {
+static int64_t ds_hold_bytes(int V, int elem, bool planes, int parts) {
   const int n = 16 / elem;
   const int64_t slots = ((int64_t)V + 2 * n - 1) / n;
   const int64_t share = (slots + parts - 1) / parts;
-  return share * (cap ? 4 * n : 16);
+  return share * (planes ? 4 * n : 16);
 }
 
-template <typename E, int kMode, bool kCap>
+template <typename E, int kMode, int kCap>
 static int launch_distill(DistillParams& p, cudaStream_t s) {
   static KernelOptIn opt_in;
-  // The fewest CTAs per row that give every SM two, of at least 1,024 slots (four loads a thread); more
-  // where the row must fit shared memory.
+  // CTAs per row: until every SM has two, of at least two batches a thread; more where a row must fit shared memory.
+  // (Splitting 2,047 rows of 50,257 over clusters of 4 to even out the last CTAs took 188 us instead of 139.)
   const int64_t slots = ((int64_t)p.V + DsSlot<E>::kN - 1) / DsSlot<E>::kN;
   const int64_t want = 2 * (int64_t)device_sm_count();
   int parts = 1;
-  while (parts < kDsMaxCluster && p.rows * parts < want && slots / (2 * parts) >= kDsThreads) parts *= 2;
-  int smem = 0;
+  while (parts < kDsMaxCluster && p.rows * parts < want && slots / (2 * parts) >= 2 * kDsBatch * kDsThreads) parts *= 2;
+  int smem = kDsRing;
   if (kMode == kDsBoth) {
-    while (parts < kDsMaxCluster && ds_hold_bytes(p.V, sizeof(E), kCap, parts) > kDsRowBytes / 4) parts *= 2;
-    const int64_t need = ds_hold_bytes(p.V, sizeof(E), kCap, parts);
+    while (parts < kDsMaxCluster && ds_hold_bytes(p.V, sizeof(E), kCap == kCapBound, parts) > kDsRowBytes / 4) parts *= 2;
+    const int64_t need = ds_hold_bytes(p.V, sizeof(E), kCap == kCapBound, parts);
     if (need > kDsRowBytes) return kStatusUnsupported;
     smem = (int)need;
   }
   if (p.rows * parts > INT32_MAX) return kStatusUnsupported;
   p.parts = parts;
-  if (!opt_in(distill_kernel<E, kMode, kCap>, kMode == kDsBoth ? kDsRowBytes : 0)) return kStatusLaunchFailed;
+  if (!opt_in(distill_kernel<E, kMode, kCap>, kMode == kDsBoth ? kDsRowBytes : kDsRing)) return kStatusLaunchFailed;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = (unsigned)parts, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
@@ -368,12 +489,16 @@ static int launch_distill(DistillParams& p, cudaStream_t s) {
   return kStatusOk;
 }
 
+template <typename E, int kMode>
+static int launch_distill_cap(DistillParams& p, cudaStream_t s) {
+  if (p.cap == 0.f) return launch_distill<E, kMode, kCapNone>(p, s);
+  return p.cap / p.tau <= kDsBoundCap ? launch_distill<E, kMode, kCapBound>(p, s) : launch_distill<E, kMode, kCapFree>(p, s);
+}
+
 template <typename E>
 static int launch_distill_mode(DistillParams& p, int mode, cudaStream_t s) {
-  const bool cap = p.cap > 0.f;
-  if (mode == kDsLoss) return cap ? launch_distill<E, kDsLoss, true>(p, s) : launch_distill<E, kDsLoss, false>(p, s);
-  if (mode == kDsGrad) return cap ? launch_distill<E, kDsGrad, true>(p, s) : launch_distill<E, kDsGrad, false>(p, s);
-  return cap ? launch_distill<E, kDsBoth, true>(p, s) : launch_distill<E, kDsBoth, false>(p, s);
+  return mode == kDsLoss ? launch_distill_cap<E, kDsLoss>(p, s)
+                         : mode == kDsGrad ? launch_distill_cap<E, kDsGrad>(p, s) : launch_distill_cap<E, kDsBoth>(p, s);
 }
 
 }  // namespace noise

@@ -87,6 +87,17 @@ struct Vec8<float> {
   __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
 };
 
+// 16 bytes of global memory into shared memory without a register; `have` false fills zeros and reads nothing.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool have = true) {
+  const int n = have ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // A kernel's opt-in to `bytes` of dynamic shared memory (and to clusters of more than 8 CTAs), made once
 // per device: the attribute belongs to the device that is current when it is set.
 struct KernelOptIn {

@@ -37,9 +37,9 @@ def _call(name, logits, ids, teacher, temperature, softcap, dloss=None, lse=None
         raise ValueError(f'{name}: 1 to {MAX_ENTRIES} entries a row and 1 to 2^30 logits, got {ids.shape[1]} and {V}')
     if not 0 < temperature < float('inf') or not 0 <= softcap < float('inf'):
         raise ValueError(f'{name}: temperature must be positive and softcap not negative, got {temperature} and {softcap}')
-    for t, what in ((dloss, 'dloss'), (lse, 'lse')):
-        if t is not None and (t.shape != (N,) or t.dtype != torch.float32):
-            raise ValueError(f'{name}: {what} must be fp32 [{N}], got {t.dtype} {tuple(t.shape)}')
+    for t, what, dtype in ((dloss, 'dloss', torch.float32), (lse, 'lse', torch.float64)):
+        if t is not None and (t.shape != (N,) or t.dtype != dtype):
+            raise ValueError(f'{name}: {what} must be {dtype} [{N}], got {t.dtype} {tuple(t.shape)}')
     if want_loss and want_grad:
         limit = int(_lib.load().noise_distill_max_vocab(DTYPE_CODES[logits.dtype], int(softcap > 0)))
         if V > limit:
@@ -48,7 +48,7 @@ def _call(name, logits, ids, teacher, temperature, softcap, dloss=None, lse=None
     device = device_index(name, logits, ids, teacher, dloss, lse)
     where = logits.device
     loss = torch.empty(N, dtype=torch.float32, device=where) if want_loss else None
-    out_lse = torch.empty(N, dtype=torch.float32, device=where) if want_loss and not want_grad else None
+    out_lse = torch.empty(N, dtype=torch.float64, device=where) if want_loss and not want_grad else None
     grad = torch.empty(N, V, dtype=logits.dtype, device=where) if want_grad else None
     if N:
         (logits, ld), (ids, ids_ld), (teacher, teacher_ld) = _matrix(logits), _matrix(ids), _matrix(teacher)
@@ -66,7 +66,8 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
                  softcap: float = 0.0):
     """Losses of logits [N, V] against the teacher's entries: ids [N, K] (int32 or int64, K up to 1,024) and their
     logits teacher [N, K]. An id outside [0, V) marks an absent entry, equal ids add up, and a row without an entry
-    above -inf has loss 0. Returns (loss fp32 [N], lse fp32 [N]); lse is what distill_backward needs."""
+    above -inf has loss 0. Returns (loss fp32 [N], lse fp64 [N]); lse is what distill_backward needs, in 64 bits because
+    all of a row's gradient shares its error."""
     return _call('distill_loss', logits, ids, teacher, temperature, softcap)[:2]
 
 
