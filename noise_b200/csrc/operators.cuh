@@ -87,6 +87,38 @@ struct Vec8<float> {
   __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
 };
 
+// n / d for n < 2^31 by a multiplication: with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, the quotient is
+// (mulhi(m, n) + n) >> s (Granlund and Montgomery, division by invariant integers).
+struct FastDiv {
+  uint32_t d, m, s;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t divisor) : d(divisor), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
+};
+
+// Four consecutive elements, aligned to their size: one 8-byte access of a 16-bit type, one 16-byte access of fp32.
+template <typename E>
+struct Vec4 {
+  uint2 w;
+  __device__ __forceinline__ void load(const E* p) { w = __ldcs(reinterpret_cast<const uint2*>(p)); }
+  __device__ __forceinline__ void store(E* p) const { __stcs(reinterpret_cast<uint2*>(p), w); }
+  __device__ __forceinline__ void get(float2 (&v)[2]) const { v[0] = unpack2<E>(w.x), v[1] = unpack2<E>(w.y); }
+  __device__ __forceinline__ void set(const float2 (&v)[2]) { w = make_uint2(pack2<E>(v[0].x, v[0].y), pack2<E>(v[1].x, v[1].y)); }
+  __device__ __forceinline__ void zero() { w = make_uint2(0u, 0u); }
+};
+template <>
+struct Vec4<float> {
+  float4 a;
+  __device__ __forceinline__ void load(const float* p) { a = __ldcs(reinterpret_cast<const float4*>(p)); }
+  __device__ __forceinline__ void store(float* p) const { __stcs(reinterpret_cast<float4*>(p), a); }
+  __device__ __forceinline__ void get(float2 (&v)[2]) const { v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w); }
+  __device__ __forceinline__ void set(const float2 (&v)[2]) { a = make_float4(v[0].x, v[0].y, v[1].x, v[1].y); }
+  __device__ __forceinline__ void zero() { a = make_float4(0.f, 0.f, 0.f, 0.f); }
+};
+
 // 16 bytes of global memory into shared memory without a register; `have` false fills zeros and reads nothing.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool have = true) {
   const int n = have ? 16 : 0;

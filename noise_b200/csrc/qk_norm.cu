@@ -11,8 +11,8 @@
 //
 // Bound: HBM. A pass reads and writes each value once (the gradient reads x and dy and writes dx; the
 // norm's factor is recomputed from x, which costs nothing beside reading it). A row belongs to
-// D / 16 lanes of one warp, each with eight values of either half, so a pair (x1, x2) never leaves its
-// lane and the mean is a shuffle over at most 16 lanes. A lane takes several heads of one token at a
+// D / 8 lanes of one warp, each with four values of either half, so a pair (x1, x2) never leaves its
+// lane and the mean is a shuffle over the row's lanes. A lane takes several heads of one token at a
 // time: their loads are in flight together and share the table's values. Query and key rows go to
 // different CTAs of one launch, so that the weight gradients need one accumulator set a thread.
 #include "operators.cuh"
@@ -27,9 +27,10 @@ struct QkSide {
   void* y;         // y, or dx in the gradient pass, strides ys
   const float* w;  // [D] or null
   int64_t xs[3], ds[3], ys[3];
-  int heads, chunks;  // chunks: groups of heads that one lane group takes at a time
-  int64_t units;      // B * T * chunks
-  int blocks;         // CTAs of the launch that work on this side
+  int heads;
+  FastDiv chunks;  // groups of heads that one lane group takes at a time
+  uint32_t units;  // B * T * chunks
+  int blocks;      // CTAs of the launch that work on this side
 };
 
 struct QkParams {
@@ -38,89 +39,95 @@ struct QkParams {
   const int* positions;
   int64_t pos_b;  // batch stride of positions (0: one row for all sequences)
   int64_t table;
-  int T, D, lanes, rotate_first;
+  FastDiv T;
+  int D, rotate_first;
   float eps;
   float* partial;  // gradient pass with weights: [blocks of both sides][D]
 };
 
-// One row's values: eight of the first half, eight of the second.
-struct Row16 {
-  float a[8], b[8];
+// A lane's values of one row: four of the first half, four of the second, in pairs (the sm_100 f32x2 arithmetic).
+struct RowPart {
+  float2 a[2], b[2];
 };
 
-__device__ __forceinline__ void rotate(Row16& r, const float (&c)[8], const float (&s)[8]) {
+__device__ __forceinline__ float2 minus(float2 v) { return make_float2(-v.x, -v.y); }
+
+__device__ __forceinline__ void rotate(RowPart& r, const float2 (&c)[2], const float2 (&s)[2]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x1 = r.a[i], x2 = r.b[i];
-    r.a[i] = fmaf(x1, c[i], x2 * s[i]);
-    r.b[i] = fmaf(x2, c[i], -x1 * s[i]);
+  for (int i = 0; i < 2; ++i) {
+    const float2 x1 = r.a[i], x2 = r.b[i];
+    r.a[i] = __ffma2_rn(x1, c[i], __fmul2_rn(x2, s[i]));
+    r.b[i] = __ffma2_rn(x2, c[i], __fmul2_rn(x1, minus(s[i])));
   }
 }
 
-__device__ __forceinline__ void rotate_back(Row16& r, const float (&c)[8], const float (&s)[8]) {
+__device__ __forceinline__ void rotate_back(RowPart& r, const float2 (&c)[2], const float2 (&s)[2]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x1 = r.a[i], x2 = r.b[i];
-    r.a[i] = fmaf(x1, c[i], -x2 * s[i]);
-    r.b[i] = fmaf(x1, s[i], x2 * c[i]);
+  for (int i = 0; i < 2; ++i) {
+    const float2 x1 = r.a[i], x2 = r.b[i];
+    r.a[i] = __ffma2_rn(x1, c[i], __fmul2_rn(x2, minus(s[i])));
+    r.b[i] = __ffma2_rn(x2, c[i], __fmul2_rn(x1, s[i]));
   }
 }
 
-// Sum over the row's lane group (a power of two of lanes; the lanes past D / 16 hold zeros).
-__device__ __forceinline__ float group_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+// Sum over the row's lane group (a power of two of lanes; the lanes past D / 8 hold zeros).
+template <int kLanes>
+__device__ __forceinline__ float group_sum(float2 t) {
+  float v = t.x + t.y;
+#pragma unroll
+  for (int o = kLanes >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-__device__ __forceinline__ float square_sum(const Row16& r) {
-  float t = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t = fmaf(r.a[i], r.a[i], fmaf(r.b[i], r.b[i], t));
-  return t;
+__device__ __forceinline__ float2 dot(const RowPart& p, const RowPart& q) {
+  float2 t = __fmul2_rn(p.a[0], q.a[0]);
+  t = __ffma2_rn(p.a[1], q.a[1], t);
+  t = __ffma2_rn(p.b[0], q.b[0], t);
+  return __ffma2_rn(p.b[1], q.b[1], t);
 }
 
-__device__ __forceinline__ float dot(const Row16& p, const Row16& q) {
-  float t = 0.f;
+__device__ __forceinline__ void scale_by(RowPart& r, const float2 (&a)[2], const float2 (&b)[2]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t = fmaf(p.a[i], q.a[i], fmaf(p.b[i], q.b[i], t));
-  return t;
+  for (int i = 0; i < 2; ++i) r.a[i] = __fmul2_rn(r.a[i], a[i]), r.b[i] = __fmul2_rn(r.b[i], b[i]);
 }
 
 constexpr int kQkThreads = 256;
 
 // IT heads of a token per lane group and step.
-template <typename E, int IT, bool kGrad>
+template <typename E, int IT, bool kGrad, int kLanes>
 __global__ void __launch_bounds__(kQkThreads) qk_norm_kernel(const __grid_constant__ QkParams p) {
   const bool key = (int)blockIdx.x >= p.side[0].blocks;
   const QkSide& S = p.side[key];
   const int block = key ? blockIdx.x - p.side[0].blocks : blockIdx.x;
-  const int lanes = p.lanes, half = p.D / 2;
+  constexpr int lanes = kLanes;
+  const int half = p.D / 2;
   const int gl = threadIdx.x & (lanes - 1);          // lane of the row's group
   const int groups = kQkThreads / lanes, group = threadIdx.x / lanes;
-  const bool on = gl * 16 < p.D;
-  const int col = on ? gl * 8 : 0;
+  const bool on = gl * 8 < p.D;
+  const int col = on ? gl * 4 : 0;
   const float inv_d = 1.0f / (float)p.D;
-  float wa[8], wb[8];
+  float2 wa[2], wb[2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    wa[i] = S.w ? __ldg(S.w + col + i) : 1.f;
-    wb[i] = S.w ? __ldg(S.w + half + col + i) : 1.f;
+  for (int i = 0; i < 2; ++i) {
+    wa[i] = S.w ? make_float2(__ldg(S.w + col + 2 * i), __ldg(S.w + col + 2 * i + 1)) : make_float2(1.f, 1.f);
+    wb[i] = S.w ? make_float2(__ldg(S.w + half + col + 2 * i), __ldg(S.w + half + col + 2 * i + 1)) : make_float2(1.f, 1.f);
   }
-  Row16 dw;
+  RowPart dw;
   if (kGrad) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dw.a[i] = dw.b[i] = 0.f;
+    for (int i = 0; i < 2; ++i) dw.a[i] = dw.b[i] = make_float2(0.f, 0.f);
   }
   // Every lane runs the same number of steps: the shuffles below need the whole warp.
-  for (int64_t u0 = (int64_t)block * groups; u0 < S.units; u0 += (int64_t)S.blocks * groups) {
-    const int64_t unit = u0 + group;
+  for (uint32_t u0 = (uint32_t)block * groups; u0 < S.units; u0 += (uint32_t)S.blocks * groups) {
+    const uint32_t unit = u0 + group;
     const bool live = on && unit < S.units;
-    const int64_t token = live ? unit / S.chunks : 0;
-    const int h0 = live ? (int)(unit - token * S.chunks) * IT : 0;
-    const int64_t b = token / p.T, t = token - b * p.T;
+    const uint32_t token = live ? S.chunks(unit) : 0;
+    const int h0 = live ? (int)(unit - token * S.chunks.d) * IT : 0;
+    const uint32_t seq = p.T(token);
+    const int64_t b = seq, t = token - seq * p.T.d;
     const E* x = reinterpret_cast<const E*>(S.x) + b * S.xs[0] + t * S.xs[1] + col;
     const E* dy = kGrad ? reinterpret_cast<const E*>(S.dy) + b * S.ds[0] + t * S.ds[1] + col : nullptr;
-    Vec8<E> va[IT], vb[IT], ga[kGrad ? IT : 1], gb[kGrad ? IT : 1];
+    Vec4<E> va[IT], vb[IT], ga[kGrad ? IT : 1], gb[kGrad ? IT : 1];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const bool have = live && h0 + i < S.heads;
@@ -132,58 +139,51 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_kernel(const __grid_consta
       }
     }
     const int64_t pos = p.positions ? (int64_t)__ldg(p.positions + b * p.pos_b + t) : t;
-    float c[8], s[8];
+    float2 c[2], s[2];
     // a position outside the table has no rotation: its rows come out as NaN
-    const bool known = pos >= 0 && pos < p.table;
-    if (known) {
-      Vec8<float> tc, ts;
-      tc.load(p.rope + pos * p.D + col), ts.load(p.rope + pos * p.D + half + col);
-      tc.get(c), ts.get(s);
+    if (pos >= 0 && pos < p.table) {
+      const float4 tc = __ldg(reinterpret_cast<const float4*>(p.rope + pos * p.D + col));
+      const float4 ts = __ldg(reinterpret_cast<const float4*>(p.rope + pos * p.D + half + col));
+      c[0] = make_float2(tc.x, tc.y), c[1] = make_float2(tc.z, tc.w);
+      s[0] = make_float2(ts.x, ts.y), s[1] = make_float2(ts.z, ts.w);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = s[i] = __int_as_float(0x7fffffff);
+      c[0] = c[1] = s[0] = s[1] = make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
     }
     E* y = reinterpret_cast<E*>(S.y) + b * S.ys[0] + t * S.ys[1] + col;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      Row16 z;
+      RowPart z;  // lanes without columns hold zeros
       va[i].get(z.a), vb[i].get(z.b);
       if (p.rotate_first) rotate(z, c, s);
-      if (!on) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z.a[j] = z.b[j] = 0.f;  // lanes without columns add nothing (not NaN)
-      }
-      const float r = rsqrtf(fmaf(group_sum(square_sum(z), lanes), inv_d, p.eps));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) z.a[j] *= r, z.b[j] *= r;
+      const float r = rsqrtf(fmaf(group_sum<kLanes>(dot(z, z)), inv_d, p.eps));
+      const float2 r2[2] = {make_float2(r, r), make_float2(r, r)};
+      scale_by(z, r2, r2);
       if constexpr (!kGrad) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z.a[j] *= wa[j], z.b[j] *= wb[j];
+        if (S.w) scale_by(z, wa, wb);
         if (!p.rotate_first) rotate(z, c, s);
       } else {
-        Row16 g;
+        RowPart g;
         ga[i].get(g.a), gb[i].get(g.b);
         if (!p.rotate_first) rotate_back(g, c, s);
-        if (!on) {
+        if (S.w) {
+          if (live && h0 + i < S.heads) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) g.a[j] = g.b[j] = 0.f;
-        }
-        if (live && h0 + i < S.heads) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            dw.a[j] = fmaf(g.a[j], z.a[j], dw.a[j]);
-            dw.b[j] = fmaf(g.b[j], z.b[j], dw.b[j]);
+            for (int j = 0; j < 2; ++j)
+              dw.a[j] = __ffma2_rn(g.a[j], z.a[j], dw.a[j]), dw.b[j] = __ffma2_rn(g.b[j], z.b[j], dw.b[j]);
           }
+          scale_by(g, wa, wb);
         }
+        const float m = group_sum<kLanes>(dot(z, g)) * -inv_d;
+        const float2 m2 = make_float2(m, m);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g.a[j] *= wa[j], g.b[j] *= wb[j];
-        const float m = group_sum(dot(z, g), lanes) * inv_d;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z.a[j] = r * (g.a[j] - z.a[j] * m), z.b[j] = r * (g.b[j] - z.b[j] * m);
+        for (int j = 0; j < 2; ++j) {
+          z.a[j] = __fmul2_rn(__ffma2_rn(z.a[j], m2, g.a[j]), r2[0]);
+          z.b[j] = __fmul2_rn(__ffma2_rn(z.b[j], m2, g.b[j]), r2[0]);
+        }
         if (p.rotate_first) rotate_back(z, c, s);
       }
       if (live && h0 + i < S.heads) {
-        Vec8<E> o;
+        Vec4<E> o;
         o.set(z.a), o.store(y + (h0 + i) * S.ys[2]);
         o.set(z.b), o.store(y + (h0 + i) * S.ys[2] + half);
       }
@@ -193,16 +193,15 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_kernel(const __grid_consta
     if (!S.w) return;
     // the CTA's sum: lanes of the same columns within a warp, then the warps in order
     __shared__ float part[kQkThreads / 32][256];
+    float sum[8] = {dw.a[0].x, dw.a[0].y, dw.a[1].x, dw.a[1].y, dw.b[0].x, dw.b[0].y, dw.b[1].x, dw.b[1].y};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      for (int o = 16; o >= lanes; o >>= 1) {
-        dw.a[i] += __shfl_xor_sync(0xffffffffu, dw.a[i], o);
-        dw.b[i] += __shfl_xor_sync(0xffffffffu, dw.b[i], o);
-      }
+#pragma unroll
+      for (int o = 16; o >= lanes; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (lane < lanes && on) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) part[warp][col + i] = dw.a[i], part[warp][half + col + i] = dw.b[i];
+      for (int i = 0; i < 4; ++i) part[warp][col + i] = sum[i], part[warp][half + col + i] = sum[4 + i];
     }
     __syncthreads();
     for (int i = threadIdx.x; i < p.D; i += kQkThreads) {
@@ -226,6 +225,7 @@ __global__ void __launch_bounds__(1024) qk_weight_sum_kernel(const float* __rest
   const int first = blockIdx.y ? blocks_q : 0, n = blockIdx.y ? blocks_k : blocks_q;
   float t = 0.f;
   if (col < D)
+#pragma unroll 8
     for (int i = warp; i < n; i += 32) t += partial[(int64_t)(first + i) * D + col];
   part[warp][lane] = t;
   __syncthreads();
@@ -239,23 +239,29 @@ __global__ void __launch_bounds__(1024) qk_weight_sum_kernel(const float* __rest
 
 int device_sm_count();
 
-// CTAs of a gradient pass: at most this many per SM in all, so that the weight sums stay short.
-constexpr int kQkGradBlocksPerSm = 8;
+// CTAs of a gradient pass with weights: at most this many per SM and side, so that the weights' sums stay short.
+constexpr int kQkGradBlocksPerSm = 3;
 constexpr int kQkMaxBlocks = 4096;
 
 // Splits one side's units over CTAs: one step each, or an even share of `cap` CTAs.
-static void qk_side(QkSide& s, int64_t tokens, int it, int lanes, int64_t cap) {
-  s.chunks = (s.heads + it - 1) / it;
-  s.units = tokens * s.chunks;
-  const int64_t groups = kQkThreads / lanes;
-  int64_t blocks = (s.units + groups - 1) / groups;
-  if (blocks > cap) blocks = cap;
-  s.blocks = (int)(blocks < 1 ? 1 : blocks);
+static bool qk_side(QkSide& s, int64_t tokens, int it, int lanes, int64_t cap) {
+  const int64_t chunks = (s.heads + it - 1) / it, units = tokens * chunks, groups = kQkThreads / lanes;
+  const int64_t blocks = min((units + groups - 1) / groups, cap);
+  if (units + blocks * groups > INT32_MAX) return false;  // unit numbers and their steps stay below 2^31
+  s.chunks = FastDiv((uint32_t)chunks), s.units = (uint32_t)units, s.blocks = (int)blocks;
+  return true;
 }
 
 template <typename E, int IT, bool kGrad>
-static void launch_qk(const QkParams& p, cudaStream_t s) {
-  qk_norm_kernel<E, IT, kGrad><<<p.side[0].blocks + p.side[1].blocks, kQkThreads, 0, s>>>(p);
+static void launch_qk(const QkParams& p, int lanes, cudaStream_t s) {
+  const int blocks = p.side[0].blocks + p.side[1].blocks;
+  switch (lanes) {
+    case 2: return qk_norm_kernel<E, IT, kGrad, 2><<<blocks, kQkThreads, 0, s>>>(p);
+    case 4: return qk_norm_kernel<E, IT, kGrad, 4><<<blocks, kQkThreads, 0, s>>>(p);
+    case 8: return qk_norm_kernel<E, IT, kGrad, 8><<<blocks, kQkThreads, 0, s>>>(p);
+    case 16: return qk_norm_kernel<E, IT, kGrad, 16><<<blocks, kQkThreads, 0, s>>>(p);
+    default: return qk_norm_kernel<E, IT, kGrad, 32><<<blocks, kQkThreads, 0, s>>>(p);
+  }
 }
 
 static bool qk_tensor_ok(const void* ptr, const int64_t* stride, int elem) {
@@ -304,27 +310,27 @@ extern "C" int noise_qk_norm_rope(const NoiseQkNorm* a, int backward, void* work
     p.side[1].xs[i] = a->k_stride[i], p.side[1].ds[i] = a->dk_stride[i], p.side[1].ys[i] = a->k_out_stride[i];
   }
   p.rope = a->rope, p.positions = a->positions, p.pos_b = a->positions_stride, p.table = a->table;
-  p.T = a->T, p.D = a->D, p.rotate_first = a->order == NOISE_ROTATE_NORM, p.eps = a->eps;
-  p.lanes = 1;
-  while (p.lanes * 16 < a->D) p.lanes *= 2;
+  p.T = FastDiv((uint32_t)a->T), p.D = a->D, p.rotate_first = a->order == NOISE_ROTATE_NORM, p.eps = a->eps;
+  int lanes = 2;
+  while (lanes * 8 < a->D) lanes *= 2;
   p.partial = reinterpret_cast<float*>(workspace);
   const int64_t tokens = (int64_t)a->B * a->T;
   const bool wide = a->dtype == NOISE_FP32;
   const int it = backward ? (wide ? 1 : 2) : (wide ? 2 : 4);
-  int64_t cap = INT32_MAX / 2;
+  // The forward and a gradient without weights take one step a CTA. Weight sums want few CTAs, each with many rows.
+  int64_t cap = INT32_MAX;
   if (weights) cap = min((int64_t)kQkMaxBlocks, (int64_t)device_sm_count() * kQkGradBlocksPerSm);
-  qk_side(p.side[0], tokens, it, p.lanes, cap);
-  qk_side(p.side[1], tokens, it, p.lanes, cap);
+  if (!qk_side(p.side[0], tokens, it, lanes, cap) || !qk_side(p.side[1], tokens, it, lanes, cap)) return kStatusUnsupported;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   LaunchScope scope(kKindOther, s, weights ? 2 : 1);
   if (!backward) {
-    if (a->dtype == NOISE_FP32) launch_qk<float, 2, false>(p, s);
-    else if (a->dtype == NOISE_BF16) launch_qk<__nv_bfloat16, 4, false>(p, s);
-    else launch_qk<__half, 4, false>(p, s);
+    if (a->dtype == NOISE_FP32) launch_qk<float, 2, false>(p, lanes, s);
+    else if (a->dtype == NOISE_BF16) launch_qk<__nv_bfloat16, 4, false>(p, lanes, s);
+    else launch_qk<__half, 4, false>(p, lanes, s);
   } else {
-    if (a->dtype == NOISE_FP32) launch_qk<float, 1, true>(p, s);
-    else if (a->dtype == NOISE_BF16) launch_qk<__nv_bfloat16, 2, true>(p, s);
-    else launch_qk<__half, 2, true>(p, s);
+    if (a->dtype == NOISE_FP32) launch_qk<float, 1, true>(p, lanes, s);
+    else if (a->dtype == NOISE_BF16) launch_qk<__nv_bfloat16, 2, true>(p, lanes, s);
+    else launch_qk<__half, 2, true>(p, lanes, s);
     if (weights)
       qk_weight_sum_kernel<<<dim3((a->D + 31) / 32, 2), 1024, 0, s>>>(p.partial, p.side[0].blocks, p.side[1].blocks, a->D,
                                                                       a->dwq, a->dwk);
