@@ -6,6 +6,8 @@
   head_error              -> noise_coordinate_differences
   reassemble              -> noise_reassemble (errT . x on tf32 tensor cores, as the reference's einsum
                              under set_float32_matmul_precision('high'))
+  exact_local_errors      -> noise_qk_norm_rope, noise_window_attention and their gradients (what local_errors estimates)
+  distill_error           -> noise_distill (the head's error against a teacher's top logits)
   CreditMemory            -> torch fp32 algebra (cuBLAS products, cuSOLVER Cholesky) at the same precision
 """
 from __future__ import annotations
@@ -18,7 +20,9 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .model import LAYERS, TENSOR_ID, VOCAB, WIDTH, Weights
+from .attention import qk_norm_rope, qk_norm_rope_backward, window_attention, window_attention_backward
+from .distill import distill_loss_grad
+from .model import HEAD_DIM, HEADS, LAYERS, TENSOR_ID, VOCAB, WIDTH, Weights
 from .population import units_that_fit, workspace, workspace_bytes
 
 HIDDEN = 4 * WIDTH
@@ -291,6 +295,20 @@ def head_error(cap: Capture, sigma: float = 0.1) -> torch.Tensor:
     return out.view(cap.B, cap.T, VOCAB)
 
 
+SOFTCAP = 15.0  # the head's soft cap (utils/model.py:204)
+
+
+def distill_error(cap: Capture, ids: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0):
+    """The captured head against a teacher's top logits instead of the targets: ids and teacher [B, T, K] -> each
+    token's distillation loss [B, T] and the head's output error [B, T, 4096], the losses' exact gradient with
+    respect to the raw logits (what head_error is to the targets' loss; reassemble turns it into lm_head's
+    gradient). Tokens whose target is ignored (< 0) have error 0."""
+    k = ids.shape[-1]
+    loss, error = distill_loss_grad(cap.logits, ids.reshape(-1, k), teacher.reshape(-1, k), temperature=temperature,
+                                    softcap=SOFTCAP, dloss=(cap.y.reshape(-1) >= 0).float())
+    return loss.view(cap.B, cap.T), error.view(cap.B, cap.T, VOCAB)
+
+
 _CONTRACT_WS: dict = {}
 
 
@@ -437,6 +455,48 @@ def local_errors(w: Weights, cap: Capture, kind: str, draws: int, targets: dict,
     return out
 
 
+def layer_window(layer: int) -> int:
+    """The attention window of a block (utils/model.py:185-191: every fourth block and the last see 2,048)."""
+    return 2048 if layer % 4 == 3 or layer == LAYERS - 1 else 1024
+
+
+def exact_local_errors(w: Weights, cap: Capture, targets: dict, kinds=tuple(LOCAL_KINDS),
+                       inputs: dict | None = None) -> dict[str, dict[str, torch.Tensor]]:
+    """The errors that local_errors estimates, without draws: {kind: {site: [B, T, width]}}, the gradients of
+    sum <targets[layer], attention output> with respect to each block's raw queries and keys, values, gate logits and
+    value-embedding rows. local_errors converges to them as its draws grow and sigma shrinks, for gamma = 1 where
+    a score is spread over tokens (its credit decays by gamma a token). Every rank gets the same errors."""
+    dev, B, T = w.device, cap.B, cap.T
+    shape = (B, T, HEADS, HEAD_DIM)
+    rope = w.rope(T)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = {kind: {} for kind in kinds}
+    for layer in range(LAYERS):
+        wanted = [kind for kind in kinds if layer in local_layers(kind)]
+        if not wanted:
+            continue
+        li = inputs[layer] if inputs is not None and layer in inputs else LocalInputs(w, cap, layer)
+        raw_q, raw_k, values = (t.view(shape) for t in (li.raw['q'], li.raw['k'], li.values))
+        q, k = qk_norm_rope(raw_q, raw_k, rope)
+        target = targets[layer].reshape(shape).bfloat16()
+        window = layer_window(layer)
+        y, lse = window_attention(q, k, values, window, status=status)
+        dq, dk, dv = window_attention_backward(target, q, k, values, y, lse, window, status=status)
+        found = {}
+        if 'q' in wanted or 'k' in wanted:
+            found['q'], found['k'] = (t.float() for t in qk_norm_rope_backward(dq, dk, raw_q, raw_k, rope)[:2])
+        found['v'] = dv = dv.float()
+        if li.z is not None:  # values = v + 2 sigmoid(z) ve, one z a head
+            gate, ve = torch.sigmoid(li.z).view(B, T, HEADS, 1), li.ve.view(shape)
+            found['ve'] = 2 * gate * dv
+            found['gate'] = (2 * gate * (1 - gate) * ve * dv).sum(-1)
+        for kind in wanted:
+            out[kind][local_site(kind, layer)] = found[kind].reshape(B, T, -1)
+    if int(status.item()):
+        raise _lib.NoiseError('exact local errors: device wait timed out')
+    return out
+
+
 def reassemble_local(w: Weights, cap: Capture, kind: str, layer: int, error: torch.Tensor,
                      inputs: LocalInputs | None = None) -> torch.Tensor:
     """Weight gradient of a local site (run.py:465-471): value embeddings by token id, else err^T x."""
@@ -470,6 +530,7 @@ class Recipe:
     memory_beta: float = 0.9
     mesa_ridge: float = 0.1
     alpha_beta: float = 0.8
+    exact_local: bool = False  # attention-internal errors from their gradients instead of draws
 
 
 def recipe(scale: float) -> Recipe:
@@ -588,10 +649,12 @@ class DUST:
             gamma = r.first_gamma if layer == 0 else 0.0
             self.targets[layer] = self._average(self._errors([f'o@{layer}'], r.hubs[layer], sigma, layer, gamma)[f'o@{layer}'])
         inputs = {layer: LocalInputs(self.w, cap, layer) for layer in range(layers)}
+        exact = exact_local_errors(self.w, cap, self.targets, tuple(r.local), inputs) if r.exact_local else None
         for kind, count in r.local.items():
             per = count // self.world
-            errs = local_errors(self.w, cap, kind, per, self.targets, self.seed, self.t, draw_offset=self.rank * per,
-                                inputs=inputs)
+            errs = exact[kind] if exact is not None else \
+                local_errors(self.w, cap, kind, per, self.targets, self.seed, self.t, draw_offset=self.rank * per,
+                             inputs=inputs)
             for (name, err), layer in zip(errs.items(), local_layers(kind)):
                 grads.views[name + '.weight'].copy_(reassemble_local(self.w, cap, kind, layer, err, inputs[layer]))
         del inputs

@@ -42,6 +42,8 @@ def main(track: str = 'val', default_scale: float = 1.0, target: float | None = 
     parser.add_argument('--steps', type=int, help='Stop after this many updates (smoke tests).')
     parser.add_argument('--eval-every', type=int, default=0, help='Untimed validation every this many updates.')
     parser.add_argument('--synthetic', action='store_true', help='Zipf(1.1) rows when the FineWeb files are absent.')
+    parser.add_argument('--exact-local', action='store_true',
+                        help='Attention-internal errors from their gradients instead of draws (how much the draws cost).')
     args = parser.parse_args()
 
     if not torch.cuda.is_available():
@@ -58,6 +60,7 @@ def main(track: str = 'val', default_scale: float = 1.0, target: float | None = 
         settings.lr = args.lr
     if args.anvil_lr is not None:
         settings.anvil_lr = args.anvil_lr
+    settings.exact_local = args.exact_local
 
     training = load_rows(args.data_dir / 'train.pt', TRAIN_ROWS, args.synthetic, seed=1)
     training = training[torch.randperm(len(training), generator=torch.Generator().manual_seed(SEED + 1))]
