@@ -60,7 +60,7 @@ SIGNATURES: dict[str, tuple] = {
                                    c_float, c_float, c_void_p]),
     'noise_fitness_workspace_bytes': (c_size_t, [c_int]),
     'noise_fitness': (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
-    'noise_update_sum_fe_adamw': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_char_p, c_void_p, c_int, c_float, c_uint32,
+    'noise_update_sum_fe_adamw': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_uint32,
                                           c_uint32, c_void_p, c_float, c_float, c_float, c_float, c_float, c_int,
                                           c_void_p, c_void_p]),
     'noise_adamw_region': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float,
