@@ -21,7 +21,9 @@
 // each item's chain (S and dP, the warps' arithmetic, the gradients' products), not a unit, so two items are in
 // flight per SM (two CTAs with one buffer of S and dP each at a head width of 64, one CTA with two buffers at 128)
 // and eight warps share an item, each with 32 rows and half of the columns.
-// P and dS are rounded to bf16, as the tensor core needs; sums are fp32.
+// P is rounded to bf16, as the tensor core needs. dS goes in as two bf16 numbers, its rounding and what that leaves (the
+// columns that dP lay in hold both): rounded once, dQ and dK were off by 2.4e-3 of their norm where the rounding of
+// the result alone makes 1.7e-3. Sums are fp32.
 //
 // Sinks are seen by every later query, so their key tiles have far more work than the others: it is dealt in
 // chunks to several CTAs that write fp32 partial sums, added in order by a last launch. Grouped heads with few
@@ -40,6 +42,8 @@ struct WindowGrad {
   float* partial;      // [slot][2][128][D] sums of split key tiles
   int sink_tiles, sink_splits, splits, slots;  // key tiles that hold sinks come first; slots per (sequence, key head)
   TileOrder keys, queries;
+  const __nv_bfloat16 *q, *dout;  // element strides {batch, token, head}, 0 where a dimension has one element
+  int64_t q_step[3], dout_step[3];
 };
 
 // Boxes of 128 rows for a CTA's own tiles, of 64 for the streamed ones.
@@ -59,6 +63,7 @@ struct WinBwd {
   static constexpr int kSmem = 1024 + kCore + YS * kStatBytes + 256;
   static constexpr uint32_t kAcc = NB * 128;  // columns: NB x (S 64, dP 64), then the gradients
   static constexpr uint32_t kTmemCols = 512 / kCtas;
+  static constexpr uint32_t kXCol = kAcc + DP;  // queries' side: Q, then dO, as 16-bit pairs
   static_assert(kAcc + 2 * DP <= kTmemCols, "S, dP and both gradients lie in tensor memory");
 };
 
@@ -200,7 +205,7 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* status = w.status;
   if (tid == 0) {
-    mbar_init(x_full, 1);
+    mbar_init(x_full, kKeys ? 1 : 8);
     for (int s = 0; s < YS; ++s) mbar_init(&y_full[s], 1), mbar_init(&y_empty[s], 1);
     for (int s = 0; s < NB; ++s) mbar_init(&s_full[s], 1), mbar_init(&p_full[s], 8);
     mbar_init(tail, 1);
@@ -224,7 +229,7 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
   if (warp == 0) {
     // ---------------- TMA producer (the whole warp) ----------------
     auto all_lanes = [](bool v) { return __all_sync(0xffffffffu, v) != 0; };
-    if (lane == 0) {
+    if (kKeys && lane == 0) {
       mbar_arrive_expect_tx(x_full, 2 * L::kXBytes);
       for (int c = 0; c < DP / 64; ++c) {
         tma_load_4d(sX + c * (kX * 128), &tm_x0, x_full, 64 * c, head, x0, b);
@@ -263,7 +268,7 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
       }
     }
     if (lane == 0) {  // copies in flight land before the CTA can exit
-      mbar_wait(x_full, 0, abort_flag, status);
+      if (kKeys) mbar_wait(x_full, 0, abort_flag, status);
       for (int j = max(0, t - YS); j < t; ++j) mbar_wait(&y_full[j % YS], (j / YS) & 1, abort_flag, status);
     }
     __syncwarp();
@@ -284,13 +289,17 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
         if (issuer) {
           const uint64_t x = smem_desc_sw128(sX), y = smem_desc_sw128(sY + st * L::kStage);
 #pragma unroll
-          for (int k = 0; k < DP / 16; ++k)
-            tc_mma_f16(tS, x + (k / 4) * (kX * 128 >> 4) + 2 * (k % 4), y + (k / 4) * (kY * 128 >> 4) + 2 * (k % 4), idesc_s,
-                       k > 0 ? 1u : 0u);
+          for (int i = 0; i < 2; ++i) {  // S, dP
 #pragma unroll
-          for (int k = 0; k < DP / 16; ++k)
-            tc_mma_f16(tS + 64, x + (L::kXBytes >> 4) + (k / 4) * (kX * 128 >> 4) + 2 * (k % 4),
-                       y + (L::kYBytes >> 4) + (k / 4) * (kY * 128 >> 4) + 2 * (k % 4), idesc_s, k > 0 ? 1u : 0u);
+            for (int k = 0; k < DP / 16; ++k) {
+              const uint64_t yk = y + i * (L::kYBytes >> 4) + (k / 4) * (kY * 128 >> 4) + 2 * (k % 4);
+              if (kKeys)
+                tc_mma_f16(tS + 64 * i, x + i * (L::kXBytes >> 4) + (k / 4) * (kX * 128 >> 4) + 2 * (k % 4), yk, idesc_s,
+                           k > 0 ? 1u : 0u);
+              else
+                tc_mma_f16_ts(tS + 64 * i, tm + L::kXCol + DP / 2 * i + 8 * k, yk, idesc_s, k > 0 ? 1u : 0u);
+            }
+          }
           tc_commit(&s_full[bf]);
         }
       }
@@ -307,6 +316,9 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
 #pragma unroll
           for (int k = 0; k < kY / 16; ++k)
             tc_mma_f16_ts(tm + L::kAcc, tD + half(k), d0 + (uint64_t)(2048 >> 4) * k, idesc_g, (u > 0 || k > 0) ? 1u : 0u);
+#pragma unroll
+          for (int k = 0; k < kY / 16; ++k)
+            tc_mma_f16_ts(tm + L::kAcc, tD + half(k) + 16, d0 + (uint64_t)(2048 >> 4) * k, idesc_g, 1u);
           if (kKeys) {
 #pragma unroll
             for (int k = 0; k < kY / 16; ++k)
@@ -339,6 +351,26 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
       nl4.x = nl4.y = have ? __ldg(st) : -INFINITY, nd4.x = nd4.y = have ? __ldg(st + 64) : 0.f;
     }
     bool ok = true;
+    if (!kKeys && set < 2) {  // set 0 brings Q's rows into tensor memory, set 1 dO's
+      const int64_t* step = set ? p.dout_step : p.q_step;
+      const __nv_bfloat16* x = (set ? p.dout : p.q) + b * step[0] + r * step[1] + head0 * step[2];
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          v[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (r < w.Tq && 32 * c + 8 * u < w.D) v[u] = *reinterpret_cast<const uint4*>(x + 32 * c + 8 * u);
+        }
+        const uint32_t words[16] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w,
+                                    v[2].x, v[2].y, v[2].z, v[2].w, v[3].x, v[3].y, v[3].z, v[3].w};
+        tmem_st16(tmem + lanes + L::kXCol + DP / 2 * set + 16 * c, words);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(x_full);
+    }
     for (int t = bf; t < items; t += NB) {
       step_to(it, t, t == bf ? begin + bf : NB);
       const int st = t % YS, y0 = it.y * kY;
@@ -350,11 +382,11 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
       const int yc = y0 + 32 * h;
       const int qlo = kKeys ? w.offset + yc : w.offset + rlo, qhi = kKeys ? qlo + 31 : w.offset + rhi;
       const int klo = kKeys ? rlo : yc, khi = kKeys ? rhi : yc + 31;
-      uint32_t pw[16], dw[16];
+      uint32_t pw[16], dw[16], lw[16];  // P, dS, and what dS's rounding leaves
       const bool none = window_none(qlo, qhi, klo, khi, w.window, w.sinks);
       if (none) {
 #pragma unroll
-        for (int u = 0; u < 16; ++u) pw[u] = dw[u] = 0u;
+        for (int u = 0; u < 16; ++u) pw[u] = dw[u] = lw[u] = 0u;
       } else {
         uint32_t s[32], d[32];
         tmem_ld32_async(tS + 32 * h, s);
@@ -380,17 +412,20 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
           const float2 ds = __fmul2_rn(pr, e);
           pw[u] = pack2<__nv_bfloat16>(pr.x, pr.y);
           dw[u] = pack2<__nv_bfloat16>(ds.x, ds.y);
+          const float2 hi = unpack2<__nv_bfloat16>(dw[u]);
+          lw[u] = pack2<__nv_bfloat16>(ds.x - hi.x, ds.y - hi.y);
         }
         if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {  // clear what is hidden, whatever it came to
 #pragma unroll
           for (int u = 0; u < 16; ++u) {
             const uint32_t two = seen >> (2 * u), keep = (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
-            pw[u] &= keep, dw[u] &= keep;
+            pw[u] &= keep, dw[u] &= keep, lw[u] &= keep;
           }
         }
       }
       if (kKeys) tmem_st16(tS + 32 * h, pw);  // over the half of S, and of dP, that this warp has read
       tmem_st16(tD + 32 * h, dw);
+      tmem_st16(tD + 32 * h + 16, lw);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -572,6 +607,10 @@ extern "C" int noise_window_attention_backward(const NoiseWindow* a, const void*
   g.stat = reinterpret_cast<const float*>(workspace), g.stat_tiles = plan.q_tiles;
   g.partial = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + plan.stat_bytes);
   g.dq = dq, g.dk = dk, g.dv = dv;
+  g.q = reinterpret_cast<const __nv_bfloat16*>(a->q), g.dout = reinterpret_cast<const __nv_bfloat16*>(dout);
+  const int64_t size[3] = {a->B, a->Tq, a->H};
+  for (int i = 0; i < 3; ++i)
+    g.q_step[i] = size[i] > 1 ? a->q_stride[i] : 0, g.dout_step[i] = size[i] > 1 ? dout_stride[i] : 0;
   g.sink_tiles = plan.sink_tiles, g.sink_splits = plan.sink_splits, g.splits = plan.splits, g.slots = plan.slots;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return a->D <= 64 ? launch_window_backward<64>(a, dout, dout_stride, g, plan, s)
