@@ -32,21 +32,38 @@ def device_index(name: str, *tensors) -> int:
 
 def launch(name: str, device: int, *args) -> None:
     """One library call on the device's current stream (the last argument of every entry point)."""
-    if device == torch.cuda.current_device():
-        # the raw handle of torch.cuda.current_stream(device), without building a Stream object
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
-    else:
+    if device != torch.cuda.current_device():
         with torch.cuda.device(device):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+            return launch(name, device, *args)
+    # the raw handle of torch.cuda.current_stream(device), without building a Stream object
+    _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
 
 
 def _pointer(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+# What the checks of a call gave, by the call's shapes, strides, types and options: a repeated call skips them.
+_CHECKED: dict = {}
+
+
+def checked(key, make):
+    found = _CHECKED.get(key)
+    if found is None:
+        if len(_CHECKED) >= 4096:
+            _CHECKED.clear()
+        found = _CHECKED[key] = make()
+    return found
+
+
+def _meta(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
 def _steps(t: torch.Tensor, broadcast: bool):
-    """Element strides {batch, token, head} if the kernels can step through t, else None: D contiguous, 16-byte
-    aligned rows, no dimension broadcast (unless allowed). A dimension of one element is never stepped along."""
+    """Element strides {batch, token, head} if the kernels can step through t, else None: D contiguous, strides of whole
+    16 bytes, no dimension broadcast (unless allowed). A dimension of one element is never stepped along. The
+    address must be 16-byte aligned besides."""
     sb, st, sh, sd = t.stride()
     B, T, H, D = t.shape
     if B == 1:
@@ -55,17 +72,16 @@ def _steps(t: torch.Tensor, broadcast: bool):
         st = 0
     if H == 1:
         sh = 0
-    if (sd != 1 and D != 1) or t.data_ptr() & 15 or (sb | st | sh) * t.element_size() & 15:
+    if (sd != 1 and D != 1) or (sb | st | sh) * t.element_size() & 15:
         return None
     if not broadcast and ((B > 1 and not sb) or (T > 1 and not st) or (H > 1 and not sh)):
         return None
     return sb, st, sh
 
 
-def _rows(t: torch.Tensor, broadcast: bool = False):
-    """t, or a contiguous copy where its layout cannot be addressed, and its steps."""
-    steps = _steps(t, broadcast)
-    if steps is None:
+def _rows(t: torch.Tensor, steps, broadcast: bool = False):
+    """t, or a contiguous copy where its layout (steps None) or its address cannot be taken, and its steps."""
+    if steps is None or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
         steps = _steps(t, broadcast)
     return t, steps
@@ -91,8 +107,7 @@ def _qk_check(q, k, rope, positions, q_weight, k_weight, order):
         raise ValueError(f'{name}: D must be a multiple of 16 up to 256 and heads at least 1, got {tuple(q.shape)}')
     if order not in ORDERS:
         raise ValueError(f'{name}: order must be one of {sorted(ORDERS)}, got {order!r}')
-    if rope.dim() != 2 or rope.shape[1] != D or not len(rope) or rope.dtype != torch.float32 or not rope.is_contiguous() \
-            or rope.data_ptr() & 15:
+    if rope.dim() != 2 or rope.shape[1] != D or not len(rope) or rope.dtype != torch.float32 or not rope.is_contiguous():
         raise ValueError(f'{name}: rope must be a contiguous fp32 [positions, {D}] table of cos | sin, got '
                          f'{rope.dtype} {tuple(rope.shape)}')
     stride = 0
@@ -112,7 +127,24 @@ def _qk_check(q, k, rope, positions, q_weight, k_weight, order):
     return B, T, H, Hk, D, stride
 
 
-_NO_STEPS = (0, 0, 0)
+def _qk_plan(q, k, rope, positions, q_weight, k_weight, order, eps):
+    """(leading fields of NoiseQkNorm, table rows, positions' stride, steps of q, of k, of contiguous results)."""
+    eps = float(eps)
+    key = ('qk', q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, rope.shape, rope.stride(), rope.dtype,
+           _meta(positions), _meta(q_weight), _meta(k_weight), order, eps)
+
+    def make():
+        B, T, H, Hk, D, stride = _qk_check(q, k, rope, positions, q_weight, k_weight, order)
+        head = (DTYPE_CODES[q.dtype], ORDERS[order], B, T, H, Hk, D, eps)
+        return head, len(rope), stride, _steps(q, True), _steps(k, True), (T * H * D, H * D, D, T * Hk * D, Hk * D, D)
+
+    plan = checked(key, make)
+    if rope.data_ptr() & 15:
+        raise ValueError('qk_norm_rope: rope must be 16-byte aligned')
+    return plan
+
+
+_NO_STEPS = (0, 0, 0, 0, 0, 0)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, *, positions: torch.Tensor | None = None,
@@ -125,22 +157,21 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, *, positi
     t row t), and a position outside the table gives NaN rows. q_weight, k_weight: fp32 [D] weights of the
     norms. out: (q_out, k_out) to write to, of any addressable layout (a cache's rows, or q and k themselves).
     Returns (q_out, k_out)."""
-    B, T, H, Hk, D, stride = _qk_check(q, k, rope, positions, q_weight, k_weight, order)
+    head, table, stride, qs, ks, out_steps = _qk_plan(q, k, rope, positions, q_weight, k_weight, order, eps)
     if out is None:
         q_out, k_out = _like(q), _like(k)
-        q_step, k_step = (T * H * D, H * D, D), (T * Hk * D, Hk * D, D)
     else:
         q_out, k_out = out
-        q_step, k_step = _steps(q_out, False), _steps(k_out, False)
+        q_step, k_step = (_steps(t, False) if t.dim() == 4 else None for t in out)
         if q_out.shape != q.shape or k_out.shape != k.shape or q_out.dtype != q.dtype or k_out.dtype != q.dtype or \
-                q_step is None or k_step is None:
+                q_step is None or k_step is None or (q_out.data_ptr() | k_out.data_ptr()) & 15:
             raise ValueError('qk_norm_rope: out must have the shapes and type of q and k, 16-byte aligned rows')
+        out_steps = q_step + k_step
     device = device_index('qk_norm_rope', q, k, rope, positions, q_weight, k_weight, q_out, k_out)
-    (q, qs), (k, ks) = _rows(q, True), _rows(k, True)
-    a = _lib.QK_NORM.pack(DTYPE_CODES[q.dtype], ORDERS[order], B, T, H, Hk, D, eps, rope.data_ptr(), len(rope),
-                          _pointer(positions), stride, _pointer(q_weight), _pointer(k_weight), q.data_ptr(), k.data_ptr(),
-                          0, 0, q_out.data_ptr(), k_out.data_ptr(), *qs, *ks, *_NO_STEPS, *_NO_STEPS, *q_step, *k_step,
-                          0, 0)
+    (q, qs), (k, ks) = _rows(q, qs, True), _rows(k, ks, True)
+    a = _lib.QK_NORM.pack(*head, rope.data_ptr(), table, _pointer(positions), stride, _pointer(q_weight),
+                          _pointer(k_weight), q.data_ptr(), k.data_ptr(), 0, 0, q_out.data_ptr(), k_out.data_ptr(), *qs, *ks,
+                          *_NO_STEPS, *out_steps, 0, 0)
     launch('noise_qk_norm_rope', device, a, 0, None, 0)
     return q_out, k_out
 
@@ -151,21 +182,21 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     """Gradients of qk_norm_rope: dq, dk are those of its results, q, k and the rest its inputs. Returns the
     gradients of (q, k, q_weight, k_weight); a weight that was not given has None. The weights' sums run in a
     fixed order."""
-    B, T, H, Hk, D, stride = _qk_check(q, k, rope, positions, q_weight, k_weight, order)
+    head, table, stride, qs, ks, out_steps = _qk_plan(q, k, rope, positions, q_weight, k_weight, order, eps)
     if dq.shape != q.shape or dk.shape != k.shape or dq.dtype != q.dtype or dk.dtype != q.dtype:
         raise ValueError('qk_norm_rope_backward: dq and dk must have the shapes and type of q and k')
     device = device_index('qk_norm_rope_backward', q, k, dq, dk, rope, positions, q_weight, k_weight)
-    (q, qs), (k, ks), (dq, dqs), (dk, dks) = _rows(q, True), _rows(k, True), _rows(dq, True), _rows(dk, True)
+    (q, qs), (k, ks) = _rows(q, qs, True), _rows(k, ks, True)
+    (dq, dqs), (dk, dks) = _rows(dq, _steps(dq, True), True), _rows(dk, _steps(dk, True), True)
     gq, gk = _like(q), _like(k)
     gwq, gwk = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
     ws, need = None, 0
     if gwq is not None or gwk is not None:
-        need = int(_lib.load().noise_qk_norm_workspace_bytes(D))
+        need = int(_lib.load().noise_qk_norm_workspace_bytes(q.shape[3]))
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    a = _lib.QK_NORM.pack(DTYPE_CODES[q.dtype], ORDERS[order], B, T, H, Hk, D, eps, rope.data_ptr(), len(rope),
-                          _pointer(positions), stride, _pointer(q_weight), _pointer(k_weight), q.data_ptr(), k.data_ptr(),
-                          dq.data_ptr(), dk.data_ptr(), gq.data_ptr(), gk.data_ptr(), *qs, *ks, *dqs, *dks,
-                          T * H * D, H * D, D, T * Hk * D, Hk * D, D, _pointer(gwq), _pointer(gwk))
+    a = _lib.QK_NORM.pack(*head, rope.data_ptr(), table, _pointer(positions), stride, _pointer(q_weight),
+                          _pointer(k_weight), q.data_ptr(), k.data_ptr(), dq.data_ptr(), dk.data_ptr(), gq.data_ptr(),
+                          gk.data_ptr(), *qs, *ks, *dqs, *dks, *out_steps, _pointer(gwq), _pointer(gwk))
     launch('noise_qk_norm_rope', device, a, 1, _pointer(ws), need)
     return gq, gk, gwq, gwk
 
@@ -216,11 +247,10 @@ def _window_check(name, q, k, v, window, sinks, lengths, offset, scale, token):
         raise ValueError(f'{name}: {Tq} queries need 1 to 2^30 keys, at least as many, got {Tk}')
     if B > 65535 or H > 65535:
         raise ValueError(f'{name}: at most 65,535 sequences and heads a call')
-    window = Tk if window is None else min(int(window), Tk)
-    sinks = min(int(sinks), Tk)
+    window, sinks = Tk if window is None else min(window, Tk), min(sinks, Tk)
     if window < 0 or sinks < 0:
         raise ValueError(f'{name}: window and sinks cannot be negative, got {window} and {sinks}')
-    scale = D ** -0.5 if scale is None else float(scale)
+    scale = D ** -0.5 if scale is None else scale
     if not 0 < scale < float('inf'):
         raise ValueError(f'{name}: scale must be positive, got {scale}')
     if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (B,) or
@@ -230,7 +260,21 @@ def _window_check(name, q, k, v, window, sinks, lengths, offset, scale, token):
         offset = Tk - Tq
     elif not 0 <= offset <= Tk - Tq:
         raise ValueError(f'{name}: offset must lie in [0, {Tk - Tq}], got {offset}')
-    return DTYPE_CODES[q.dtype], B, Tq, Tk, H, Hk, D, int(offset), window, sinks, scale
+    return DTYPE_CODES[q.dtype], B, Tq, Tk, H, Hk, D, offset, window, sinks, scale
+
+
+def _window_plan(name, q, k, v, window, sinks, lengths, offset, scale, token):
+    """(leading fields of NoiseWindow, steps of q, k, v)."""
+    window, offset = (n if n is None else int(n) for n in (window, offset))
+    sinks, scale = int(sinks), scale if scale is None else float(scale)
+    key = (name, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, _meta(lengths),
+           window, sinks, offset, scale)
+
+    def make():
+        head = _window_check(name, q, k, v, window, sinks, lengths, offset, scale, token)
+        return head, _steps(q.unsqueeze(1) if token else q, False), _steps(k, False), _steps(v, False)
+
+    return checked(key, make)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int | None, sinks: int = 0, *,
@@ -245,14 +289,14 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     status: an int32 word that a device wait which ran out sets; without one the call waits for the
     GPU and checks its own. Returns (out [B, Tq, H, D], lse fp32 [B, H, Tq])."""
     name = 'window_attention'
-    head = _window_check(name, q, k, v, window, sinks, lengths, offset, scale, False)
+    head, qs, ks, vs = _window_plan(name, q, k, v, window, sinks, lengths, offset, scale, False)
     st = _Status(name, status)
     device = device_index(name, q, k, v, lengths)
     out = _like(q)
     lse = torch.empty((head[1], head[4], head[2]), dtype=torch.float32, device=q.device)
     if not out.numel():
         return out, lse
-    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
+    (q, qs), (k, ks), (v, vs) = _rows(q, qs), _rows(k, ks), _rows(v, vs)
     a = _lib.WINDOW.pack(*head, _pointer(lengths), q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs,
                          out.data_ptr(), lse.data_ptr())
     launch('noise_window_attention', device, a, st.pointer(device))
@@ -267,7 +311,7 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     """Gradients of window_attention (bf16): dout is out's, and out, lse are what it returned for the same
     arguments. Padding rows get zeros. Sums run in a fixed order. Returns (dq, dk, dv)."""
     name = 'window_attention_backward'
-    head = _window_check(name, q, k, v, window, sinks, lengths, offset, scale, False)
+    head, qs, ks, vs = _window_plan(name, q, k, v, window, sinks, lengths, offset, scale, False)
     if q.dtype != torch.bfloat16:
         raise ValueError(f'{name}: bf16 only, got {q.dtype}')
     if dout.shape != q.shape or out.shape != q.shape or dout.dtype != q.dtype or out.dtype != q.dtype:
@@ -279,7 +323,7 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     if not q.numel():
         return torch.empty_like(q), torch.zeros_like(k), torch.zeros_like(v)
     dq, dk, dv = _like(q), _like(k), _like(v)
-    (q, qs), (k, ks), (v, vs), (dout, gs) = _rows(q), _rows(k), _rows(v), _rows(dout)
+    (q, qs), (k, ks), (v, vs), (dout, gs) = _rows(q, qs), _rows(k, ks), _rows(v, vs), _rows(dout, _steps(dout, False))
     out, lse = out.contiguous(), lse.contiguous()
     if out.data_ptr() & 15:
         out = out.clone()
@@ -301,14 +345,15 @@ def window_attention_token(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, le
     name = 'window_attention_token'
     if lengths is None:
         raise ValueError(f'{name}: lengths are required')
-    head = _window_check(name, q, k, v, window, sinks, lengths, None, scale, True)
+    head, qs, ks, vs = _window_plan(name, q, k, v, window, sinks, lengths, None, scale, True)
     device = device_index(name, q, k, v, lengths)
     out = _like(q)
     if not out.numel():
         return out
-    q4, qs = _rows(q.unsqueeze(1))
-    (k, ks), (v, vs) = _rows(k), _rows(v)
-    a = _lib.WINDOW.pack(*head, lengths.data_ptr(), q4.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs,
+    if qs is None or q.data_ptr() & 15:
+        q, qs = q.clone(memory_format=torch.contiguous_format), (q.shape[1] * q.shape[2], 0, q.shape[2])
+    (k, ks), (v, vs) = _rows(k, ks), _rows(v, vs)
+    a = _lib.WINDOW.pack(*head, lengths.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs,
                          out.data_ptr(), 0)
     launch('noise_window_token', device, a)
     return out

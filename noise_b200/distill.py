@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .attention import DTYPE_CODES, _pointer, device_index, launch
+from .attention import DTYPE_CODES, _meta, _pointer, checked, device_index, launch
 
 MAX_ENTRIES = 1024
 
@@ -24,7 +24,7 @@ def _matrix(t: torch.Tensor):
     return t, t.stride(0) if rows > 1 else cols
 
 
-def _call(name, logits, ids, teacher, temperature, softcap, dloss=None, lse=None, want_loss=True, want_grad=False):
+def _check(name, logits, ids, teacher, temperature, softcap, dloss, lse, fused):
     if logits.dim() != 2 or ids.dim() != 2 or teacher.shape != ids.shape or len(ids) != len(logits):
         raise ValueError(f'{name}: logits [N, V], ids and teacher [N, K] expected, got {tuple(logits.shape)}, '
                          f'{tuple(ids.shape)} and {tuple(teacher.shape)}')
@@ -40,11 +40,19 @@ def _call(name, logits, ids, teacher, temperature, softcap, dloss=None, lse=None
     for t, what, dtype in ((dloss, 'dloss', torch.float32), (lse, 'lse', torch.float64)):
         if t is not None and (t.shape != (N,) or t.dtype != dtype):
             raise ValueError(f'{name}: {what} must be {dtype} [{N}], got {t.dtype} {tuple(t.shape)}')
-    if want_loss and want_grad:
+    if fused:
         limit = int(_lib.load().noise_distill_max_vocab(DTYPE_CODES[logits.dtype], int(softcap > 0)))
         if V > limit:
             raise ValueError(f'{name}: loss and gradient in one pass take at most {limit} logits a row of {logits.dtype}, '
                              f'got {V}; use distill_loss and distill_backward')
+    return DTYPE_CODES[logits.dtype], DTYPE_CODES[teacher.dtype], ids.dtype == torch.int64, V, ids.shape[1]
+
+
+def _call(name, logits, ids, teacher, temperature, softcap, dloss=None, lse=None, want_loss=True, want_grad=False):
+    temperature, softcap = float(temperature), float(softcap)
+    key = (name, _meta(logits), _meta(ids), _meta(teacher), temperature, softcap, _meta(dloss), _meta(lse))
+    head = checked(key, lambda: _check(name, logits, ids, teacher, temperature, softcap, dloss, lse, want_loss and want_grad))
+    N, V = logits.shape
     device = device_index(name, logits, ids, teacher, dloss, lse)
     where = logits.device
     loss = torch.empty(N, dtype=torch.float32, device=where) if want_loss else None
@@ -54,8 +62,7 @@ def _call(name, logits, ids, teacher, temperature, softcap, dloss=None, lse=None
         (logits, ld), (ids, ids_ld), (teacher, teacher_ld) = _matrix(logits), _matrix(ids), _matrix(teacher)
         dloss = None if dloss is None else dloss.contiguous()
         lse = None if lse is None else lse.contiguous()
-        a = _lib.DISTILL.pack(DTYPE_CODES[logits.dtype], DTYPE_CODES[teacher.dtype], ids.dtype == torch.int64, V,
-                              ids.shape[1], temperature, softcap, N, ld, ids_ld, teacher_ld, V, logits.data_ptr(),
+        a = _lib.DISTILL.pack(*head, temperature, softcap, N, ld, ids_ld, teacher_ld, V, logits.data_ptr(),
                               ids.data_ptr(), teacher.data_ptr(), _pointer(dloss), _pointer(lse), _pointer(loss),
                               _pointer(out_lse), _pointer(grad))
         launch('noise_distill', device, a)
