@@ -40,7 +40,7 @@ struct QkParams {
   int64_t pos_b;  // batch stride of positions (0: one row for all sequences)
   int64_t table;
   FastDiv T;
-  int D, rotate_first;
+  int D;
   float eps;
   float* partial;  // gradient pass with weights: [blocks of both sides][D]
 };
@@ -50,30 +50,20 @@ struct RowPart {
   float2 a[2], b[2];
 };
 
-__device__ __forceinline__ float2 minus(float2 v) { return make_float2(-v.x, -v.y); }
-
-__device__ __forceinline__ void rotate(RowPart& r, const float2 (&c)[2], const float2 (&s)[2]) {
+// R with ns = -s; its transpose with s and ns exchanged.
+__device__ __forceinline__ void rotate(RowPart& r, const float2 (&c)[2], const float2 (&s)[2], const float2 (&ns)[2]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float2 x1 = r.a[i], x2 = r.b[i];
     r.a[i] = __ffma2_rn(x1, c[i], __fmul2_rn(x2, s[i]));
-    r.b[i] = __ffma2_rn(x2, c[i], __fmul2_rn(x1, minus(s[i])));
+    r.b[i] = __ffma2_rn(x2, c[i], __fmul2_rn(x1, ns[i]));
   }
 }
 
-__device__ __forceinline__ void rotate_back(RowPart& r, const float2 (&c)[2], const float2 (&s)[2]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float2 x1 = r.a[i], x2 = r.b[i];
-    r.a[i] = __ffma2_rn(x1, c[i], __fmul2_rn(x2, minus(s[i])));
-    r.b[i] = __ffma2_rn(x2, c[i], __fmul2_rn(x1, s[i]));
-  }
-}
-
-// Sum over the row's lane group (a power of two of lanes; the lanes past D / 8 hold zeros).
+// Sum over those of the row's lane group (a power of two of lanes) that are on: the ones below D / 8.
 template <int kLanes>
-__device__ __forceinline__ float group_sum(float2 t) {
-  float v = t.x + t.y;
+__device__ __forceinline__ float group_sum(float2 t, bool on) {
+  float v = on ? t.x + t.y : 0.f;
 #pragma unroll
   for (int o = kLanes >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -94,8 +84,8 @@ __device__ __forceinline__ void scale_by(RowPart& r, const float2 (&a)[2], const
 constexpr int kQkThreads = 256;
 
 // IT heads of a token per lane group and step.
-template <typename E, int IT, bool kGrad, int kLanes>
-__global__ void __launch_bounds__(kQkThreads) qk_norm_kernel(const __grid_constant__ QkParams p) {
+template <typename E, int IT, bool kGrad, bool kRotateFirst, int kLanes>
+__global__ void __launch_bounds__(kQkThreads, 4) qk_norm_kernel(const __grid_constant__ QkParams p) {
   const bool key = (int)blockIdx.x >= p.side[0].blocks;
   const QkSide& S = p.side[key];
   const int block = key ? blockIdx.x - p.side[0].blocks : blockIdx.x;
@@ -119,27 +109,27 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_kernel(const __grid_consta
   }
   // Every lane runs the same number of steps: the shuffles below need the whole warp.
   for (uint32_t u0 = (uint32_t)block * groups; u0 < S.units; u0 += (uint32_t)S.blocks * groups) {
-    const uint32_t unit = u0 + group;
-    const bool live = on && unit < S.units;
-    const uint32_t token = live ? S.chunks(unit) : 0;
-    const int h0 = live ? (int)(unit - token * S.chunks.d) * IT : 0;
-    const uint32_t seq = p.T(token);
-    const int64_t b = seq, t = token - seq * p.T.d;
-    const E* x = reinterpret_cast<const E*>(S.x) + b * S.xs[0] + t * S.xs[1] + col;
-    const E* dy = kGrad ? reinterpret_cast<const E*>(S.dy) + b * S.ds[0] + t * S.ds[1] + col : nullptr;
+    // Lanes without columns and groups without a unit load what others load too (unit 0, columns 0): nothing but
+    // their sums and stores has to be held back. So do rows behind the last head of a token.
+    const bool live = u0 + group < S.units;
+    const uint32_t unit = live ? u0 + group : 0;
+    const uint32_t token = S.chunks(unit), h0 = (unit - token * S.chunks.d) * IT;
+    const uint32_t b = p.T(token), t = token - b * p.T.d;
+    const int heads = live && on ? S.heads - (int)h0 : 0;  // rows this lane works for
+    const E* x = reinterpret_cast<const E*>(S.x) + b * S.xs[0] + t * S.xs[1] + h0 * S.xs[2] + col;
+    const E* dy = kGrad ? reinterpret_cast<const E*>(S.dy) + b * S.ds[0] + t * S.ds[1] + h0 * S.ds[2] + col : nullptr;
     Vec4<E> va[IT], vb[IT], ga[kGrad ? IT : 1], gb[kGrad ? IT : 1];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const bool have = live && h0 + i < S.heads;
-      va[i].zero(), vb[i].zero();
-      if (have) va[i].load(x + (h0 + i) * S.xs[2]), vb[i].load(x + (h0 + i) * S.xs[2] + half);
-      if constexpr (kGrad) {
-        ga[i].zero(), gb[i].zero();
-        if (have) ga[i].load(dy + (h0 + i) * S.ds[2]), gb[i].load(dy + (h0 + i) * S.ds[2] + half);
+      va[i].load(x), vb[i].load(x + half);
+      if constexpr (kGrad) ga[i].load(dy), gb[i].load(dy + half);
+      if (i + 1 < S.heads - (int)h0) {
+        x += S.xs[2];
+        if constexpr (kGrad) dy += S.ds[2];
       }
     }
     const int64_t pos = p.positions ? (int64_t)__ldg(p.positions + b * p.pos_b + t) : t;
-    float2 c[2], s[2];
+    float2 c[2], s[2], ns[2];
     // a position outside the table has no rotation: its rows come out as NaN
     if (pos >= 0 && pos < p.table) {
       const float4 tc = __ldg(reinterpret_cast<const float4*>(p.rope + pos * p.D + col));
@@ -149,43 +139,46 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_kernel(const __grid_consta
     } else {
       c[0] = c[1] = s[0] = s[1] = make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
     }
-    E* y = reinterpret_cast<E*>(S.y) + b * S.ys[0] + t * S.ys[1] + col;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ns[i] = make_float2(-s[i].x, -s[i].y);
+    E* y = reinterpret_cast<E*>(S.y) + b * S.ys[0] + t * S.ys[1] + h0 * S.ys[2] + col;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      RowPart z;  // lanes without columns hold zeros
+      RowPart z;
       va[i].get(z.a), vb[i].get(z.b);
-      if (p.rotate_first) rotate(z, c, s);
-      const float r = rsqrtf(fmaf(group_sum<kLanes>(dot(z, z)), inv_d, p.eps));
+      if (kRotateFirst) rotate(z, c, s, ns);
+      const float r = rsqrtf(fmaf(group_sum<kLanes>(dot(z, z), on), inv_d, p.eps));
       const float2 r2[2] = {make_float2(r, r), make_float2(r, r)};
       scale_by(z, r2, r2);
       if constexpr (!kGrad) {
         if (S.w) scale_by(z, wa, wb);
-        if (!p.rotate_first) rotate(z, c, s);
+        if (!kRotateFirst) rotate(z, c, s, ns);
       } else {
         RowPart g;
         ga[i].get(g.a), gb[i].get(g.b);
-        if (!p.rotate_first) rotate_back(g, c, s);
+        if (!kRotateFirst) rotate(g, c, ns, s);
         if (S.w) {
-          if (live && h0 + i < S.heads) {
+          if (i < heads) {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
               dw.a[j] = __ffma2_rn(g.a[j], z.a[j], dw.a[j]), dw.b[j] = __ffma2_rn(g.b[j], z.b[j], dw.b[j]);
           }
           scale_by(g, wa, wb);
         }
-        const float m = group_sum<kLanes>(dot(z, g)) * -inv_d;
+        const float m = group_sum<kLanes>(dot(z, g), on) * -inv_d;
         const float2 m2 = make_float2(m, m);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           z.a[j] = __fmul2_rn(__ffma2_rn(z.a[j], m2, g.a[j]), r2[0]);
           z.b[j] = __fmul2_rn(__ffma2_rn(z.b[j], m2, g.b[j]), r2[0]);
         }
-        if (p.rotate_first) rotate_back(z, c, s);
+        if (kRotateFirst) rotate(z, c, ns, s);
       }
-      if (live && h0 + i < S.heads) {
+      if (i < heads) {
         Vec4<E> o;
-        o.set(z.a), o.store(y + (h0 + i) * S.ys[2]);
-        o.set(z.b), o.store(y + (h0 + i) * S.ys[2] + half);
+        o.set(z.a), o.store(y);
+        o.set(z.b), o.store(y + half);
+        y += S.ys[2];
       }
     }
   }
@@ -239,9 +232,10 @@ __global__ void __launch_bounds__(1024) qk_weight_sum_kernel(const float* __rest
 
 int device_sm_count();
 
-// CTAs of a gradient pass with weights: at most this many per SM and side, so that the weights' sums stay short.
-constexpr int kQkGradBlocksPerSm = 3;
-constexpr int kQkMaxBlocks = 4096;
+// A gradient pass with weights runs in one wave of CTAs, dealt to the two sides by their work, so that there are
+// few sums of weight gradients to add up.
+constexpr int kQkBlocksPerSm = 4;
+constexpr int kQkMaxBlocks = 4096;  // of both sides
 
 // Splits one side's units over CTAs: one step each, or an even share of `cap` CTAs.
 static bool qk_side(QkSide& s, int64_t tokens, int it, int lanes, int64_t cap) {
@@ -252,16 +246,21 @@ static bool qk_side(QkSide& s, int64_t tokens, int it, int lanes, int64_t cap) {
   return true;
 }
 
-template <typename E, int IT, bool kGrad>
+template <typename E, int IT, bool kGrad, bool kRotateFirst>
 static void launch_qk(const QkParams& p, int lanes, cudaStream_t s) {
   const int blocks = p.side[0].blocks + p.side[1].blocks;
   switch (lanes) {
-    case 2: return qk_norm_kernel<E, IT, kGrad, 2><<<blocks, kQkThreads, 0, s>>>(p);
-    case 4: return qk_norm_kernel<E, IT, kGrad, 4><<<blocks, kQkThreads, 0, s>>>(p);
-    case 8: return qk_norm_kernel<E, IT, kGrad, 8><<<blocks, kQkThreads, 0, s>>>(p);
-    case 16: return qk_norm_kernel<E, IT, kGrad, 16><<<blocks, kQkThreads, 0, s>>>(p);
-    default: return qk_norm_kernel<E, IT, kGrad, 32><<<blocks, kQkThreads, 0, s>>>(p);
+    case 2: return qk_norm_kernel<E, IT, kGrad, kRotateFirst, 2><<<blocks, kQkThreads, 0, s>>>(p);
+    case 4: return qk_norm_kernel<E, IT, kGrad, kRotateFirst, 4><<<blocks, kQkThreads, 0, s>>>(p);
+    case 8: return qk_norm_kernel<E, IT, kGrad, kRotateFirst, 8><<<blocks, kQkThreads, 0, s>>>(p);
+    case 16: return qk_norm_kernel<E, IT, kGrad, kRotateFirst, 16><<<blocks, kQkThreads, 0, s>>>(p);
+    default: return qk_norm_kernel<E, IT, kGrad, kRotateFirst, 32><<<blocks, kQkThreads, 0, s>>>(p);
   }
+}
+
+template <typename E, int IT, bool kGrad>
+static void launch_qk(const QkParams& p, bool rotate_first, int lanes, cudaStream_t s) {
+  rotate_first ? launch_qk<E, IT, kGrad, true>(p, lanes, s) : launch_qk<E, IT, kGrad, false>(p, lanes, s);
 }
 
 static bool qk_tensor_ok(const void* ptr, const int64_t* stride, int elem) {
@@ -276,7 +275,7 @@ static bool qk_tensor_ok(const void* ptr, const int64_t* stride, int elem) {
 using namespace noise;
 
 extern "C" int64_t noise_qk_norm_workspace_bytes(int D) {
-  return D < 16 || D > 256 ? -1 : (int64_t)2 * kQkMaxBlocks * D * 4;
+  return D < 16 || D > 256 ? -1 : (int64_t)kQkMaxBlocks * D * 4;
 }
 
 extern "C" int noise_qk_norm_rope(const NoiseQkNorm* a, int backward, void* workspace, size_t workspace_bytes,
@@ -310,27 +309,32 @@ extern "C" int noise_qk_norm_rope(const NoiseQkNorm* a, int backward, void* work
     p.side[1].xs[i] = a->k_stride[i], p.side[1].ds[i] = a->dk_stride[i], p.side[1].ys[i] = a->k_out_stride[i];
   }
   p.rope = a->rope, p.positions = a->positions, p.pos_b = a->positions_stride, p.table = a->table;
-  p.T = FastDiv((uint32_t)a->T), p.D = a->D, p.rotate_first = a->order == NOISE_ROTATE_NORM, p.eps = a->eps;
+  p.T = FastDiv((uint32_t)a->T), p.D = a->D, p.eps = a->eps;
   int lanes = 2;
   while (lanes * 8 < a->D) lanes *= 2;
   p.partial = reinterpret_cast<float*>(workspace);
   const int64_t tokens = (int64_t)a->B * a->T;
   const bool wide = a->dtype == NOISE_FP32;
   const int it = backward ? (wide ? 1 : 2) : (wide ? 2 : 4);
-  // The forward and a gradient without weights take one step a CTA. Weight sums want few CTAs, each with many rows.
-  int64_t cap = INT32_MAX;
-  if (weights) cap = min((int64_t)kQkMaxBlocks, (int64_t)device_sm_count() * kQkGradBlocksPerSm);
-  if (!qk_side(p.side[0], tokens, it, lanes, cap) || !qk_side(p.side[1], tokens, it, lanes, cap)) return kStatusUnsupported;
+  // The forward and a gradient without weights take one step a CTA.
+  int64_t cap_q = INT32_MAX, cap_k = INT32_MAX;
+  if (weights) {
+    const int64_t all = min(kQkMaxBlocks, device_sm_count() * kQkBlocksPerSm);
+    const int64_t q = (a->H + it - 1) / it, k = (a->Hk + it - 1) / it;
+    cap_k = max((int64_t)1, all * k / (q + k)), cap_q = all - cap_k;
+  }
+  if (!qk_side(p.side[0], tokens, it, lanes, cap_q) || !qk_side(p.side[1], tokens, it, lanes, cap_k))
+    return kStatusUnsupported;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   LaunchScope scope(kKindOther, s, weights ? 2 : 1);
   if (!backward) {
-    if (a->dtype == NOISE_FP32) launch_qk<float, 2, false>(p, lanes, s);
-    else if (a->dtype == NOISE_BF16) launch_qk<__nv_bfloat16, 4, false>(p, lanes, s);
-    else launch_qk<__half, 4, false>(p, lanes, s);
+    if (a->dtype == NOISE_FP32) launch_qk<float, 2, false>(p, a->order == NOISE_ROTATE_NORM, lanes, s);
+    else if (a->dtype == NOISE_BF16) launch_qk<__nv_bfloat16, 4, false>(p, a->order == NOISE_ROTATE_NORM, lanes, s);
+    else launch_qk<__half, 4, false>(p, a->order == NOISE_ROTATE_NORM, lanes, s);
   } else {
-    if (a->dtype == NOISE_FP32) launch_qk<float, 1, true>(p, lanes, s);
-    else if (a->dtype == NOISE_BF16) launch_qk<__nv_bfloat16, 2, true>(p, lanes, s);
-    else launch_qk<__half, 2, true>(p, lanes, s);
+    if (a->dtype == NOISE_FP32) launch_qk<float, 1, true>(p, a->order == NOISE_ROTATE_NORM, lanes, s);
+    else if (a->dtype == NOISE_BF16) launch_qk<__nv_bfloat16, 2, true>(p, a->order == NOISE_ROTATE_NORM, lanes, s);
+    else launch_qk<__half, 2, true>(p, a->order == NOISE_ROTATE_NORM, lanes, s);
     if (weights)
       qk_weight_sum_kernel<<<dim3((a->D + 31) / 32, 2), 1024, 0, s>>>(p.partial, p.side[0].blocks, p.side[1].blocks, a->D,
                                                                       a->dwq, a->dwk);
