@@ -251,8 +251,8 @@ def _window_check(name, q, k, v, window, sinks, lengths, offset, scale, token):
     if window < 0 or sinks < 0:
         raise ValueError(f'{name}: window and sinks cannot be negative, got {window} and {sinks}')
     scale = D ** -0.5 if scale is None else scale
-    if not 0 < scale < float('inf'):
-        raise ValueError(f'{name}: scale must be positive, got {scale}')
+    if not 2.0 ** -100 <= scale <= 2.0 ** 100:
+        raise ValueError(f'{name}: scale must lie in [2^-100, 2^100], got {scale}')
     if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (B,) or
                                 (B > 1 and lengths.stride(0) != 1)):
         raise ValueError(f'{name}: lengths must be contiguous int32 [{B}], got {lengths.dtype} {tuple(lengths.shape)}')

@@ -251,6 +251,17 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(const void* tile) {
   return d;
 }
 
+// Shared-memory descriptor for a K-major operand of 16 columns without a swizzle: rows of 16 bytes, one after the other,
+// with the first eight columns, and those with the last eight `second` bytes behind them.
+__device__ __forceinline__ uint64_t smem_desc_rows16(const void* tile, uint32_t second) {
+  uint64_t d = 0;
+  d |= ((uint64_t)smem_u32(tile) >> 4) & 0x3FFFull;
+  d |= (uint64_t)(second >> 4) << 16;  // leading byte offset: the other eight columns
+  d |= (uint64_t)(128 >> 4) << 32;     // stride byte offset: the next eight rows
+  d |= (uint64_t)1 << 46;
+  return d;
+}
+
 // Shared-memory descriptor for an MN-major operand tile written by TMA with 128-byte swizzle:
 // 128-byte rows along K, N (or M) contiguous inside a row, 8-row groups 1024 bytes apart. The
 // leading byte offset (stride between 64-element MN blocks) is set equal to the stride byte offset

@@ -423,7 +423,7 @@ bool window_operand_ok(const void* ptr, const int64_t* stride, int B, int T, int
 
 int check_window(const NoiseWindow* a, bool token) {
   if (!a || a->B < 0 || a->Tk < 1 || a->H < 1 || a->Hk < 1 || a->H % a->Hk || a->window < 0 || a->sinks < 0 ||
-      !(a->scale > 0.f))
+      !(a->scale >= 0x1p-100f && a->scale <= 0x1p100f))
     return kStatusBadArgument;
   if (a->dtype != NOISE_BF16 && a->dtype != NOISE_FP16) return kStatusUnsupported;
   if (a->D < 8 || a->D > 128 || a->D % 8) return kStatusUnsupported;

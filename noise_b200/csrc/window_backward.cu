@@ -17,12 +17,15 @@
 //   P and dS, as 16-bit pairs over the columns that S and dP lay in, are the A operands of
 //   keys' side (X = K, V; Y = Q, dO; rows are keys):     dV += P Y1, dK += dS Y0
 //   queries' side (X = Q, dO; Y = K, V; rows are queries): dQ += dS Y0
-// with Y0, Y1 read a second time, now as MN-major B operands, from the same shared memory. What bounds the kernel is
+// with Y0, Y1 read a second time, now as MN-major B operands, from the same shared memory. On the keys' side lse and Delta
+// belong to columns: one more product, of a row of ones with their three bf16 parts (24 bits), puts -lse / scale under S
+// and -Delta under dP. Read from shared memory by every thread instead they took turns with the tensor core's own reads:
+// 240 us against 217 for both sides at 8 x 2,048 tokens, 8 heads of 64, window 1,024. What bounds the kernel is
 // each item's chain (S and dP, the warps' arithmetic, the gradients' products), not a unit, so two items are in
 // flight per SM (two CTAs with one buffer of S and dP each at a head width of 64, one CTA with two buffers at 128)
 // and eight warps share an item, each with 32 rows and half of the columns.
-// P is rounded to bf16, as the tensor core needs. dS goes in as two bf16 numbers, its rounding and what that leaves (the
-// columns that dP lay in hold both): rounded once, dQ and dK were off by 2.4e-3 of their norm where the rounding of
+// P is rounded to bf16, as the tensor core needs. dS goes in as two bf16 numbers, its upper half (cut, which costs one
+// permute a pair) and the rest rounded, 16 bits in all (the columns that dP lay in hold both): rounded to one, dQ and dK were off by 2.4e-3 of their norm where the rounding of
 // the result alone makes 1.7e-3. Sums are fp32.
 //
 // Sinks are seen by every later query, so their key tiles have far more work than the others: it is dealt in
@@ -37,6 +40,7 @@ namespace noise {
 struct WindowGrad {
   WindowParams w;
   const float* stat;  // [B, H, tiles][2][64]: -lse log2(e), then -Delta; padding rows hold (-inf, 0)
+  const uint4* adds;  // [B, H, tiles][2][64]: -lse / scale, then -Delta, in three bf16 parts; padding rows hold zeros
   int stat_tiles;
   void *dq, *dk, *dv;  // contiguous [B, T, heads, D]
   float* partial;      // [slot][2][128][D] sums of split key tiles
@@ -51,16 +55,19 @@ struct WindowMaps {
   CUtensorMap k128, v128, q64, o64, q128, o128, k64, v64;
 };
 
+// The addends of S and dP: rows of eight bf16, 64 rows each.
+constexpr int kAddBytes = 2 * 64 * 16;
+
 template <int DP>
 struct WinBwd {
   static constexpr int kX = 128, kY = 64, YS = 3;
   static constexpr int NB = DP == 64 ? 1 : 2, kCtas = DP == 64 ? 2 : 1;
   static constexpr int kSets = 2 * NB;  // sets of four warps: each buffer's columns are shared by two
   static constexpr int kThreads = (2 + 4 * kSets) * 32;
-  static constexpr int kXBytes = kX * DP * 2, kYBytes = kY * DP * 2, kStatBytes = 512;
-  static constexpr int kStage = 2 * kYBytes;
-  static constexpr int kCore = 2 * kXBytes + YS * kStage;
-  static constexpr int kSmem = 1024 + kCore + YS * kStatBytes + 256;
+  static constexpr int kXBytes = kX * DP * 2, kYBytes = kY * DP * 2, kStage = 2 * kYBytes;
+  static constexpr int kAdds = (YS + 1) * 2 * kAddBytes;  // the streamed tiles' addends, ones; each with zeros behind it
+  static constexpr int kCore = kAdds + 2 * kXBytes + YS * kStage;
+  static constexpr int kSmem = 1024 + kCore + 256;
   static constexpr uint32_t kAcc = NB * 128;  // columns: NB x (S 64, dP 64), then the gradients
   static constexpr uint32_t kTmemCols = 512 / kCtas;
   static constexpr uint32_t kXCol = kAcc + DP;  // queries' side: Q, then dO, as 16-bit pairs
@@ -74,15 +81,25 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+// v as the sum of three bf16 numbers (24 bits), in the first places of a row of eight.
+__device__ __forceinline__ uint4 three_parts(float v) {
+  const __nv_bfloat16 a = __float2bfloat16_rn(v);
+  const float rest = v - __bfloat162float(a);
+  const __nv_bfloat16 b = __float2bfloat16_rn(rest);
+  return make_uint4(__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16,
+                    __bfloat16_as_ushort(__float2bfloat16_rn(rest - __bfloat162float(b))), 0u, 0u);
+}
+
 // Delta and -lse of 64 query rows of one head: D / 8 lanes a row, 16 bytes a lane.
 __global__ void __launch_bounds__(256) window_stats_kernel(const __nv_bfloat16* __restrict__ o,
                                                            const __nv_bfloat16* __restrict__ g, int64_t g_b, int64_t g_t,
                                                            int64_t g_h, const __grid_constant__ WindowParams p,
-                                                           float* __restrict__ stat) {
+                                                           float* __restrict__ stat, uint4* __restrict__ adds) {
   const int tile = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
   const int rows = min(p.Tq, window_length(p, b) - p.offset);
   const int lane = threadIdx.x & 15, first = threadIdx.x >> 4;  // 16 lanes a row
-  float* out = stat + (((int64_t)b * p.H + head) * gridDim.x + tile) * 128;
+  const int64_t at = (((int64_t)b * p.H + head) * gridDim.x + tile) * 128;
+  float* out = stat + at;
 #pragma unroll
   for (int r = first; r < 64; r += 16) {
     const int i = tile * 64 + r;
@@ -99,8 +116,11 @@ __global__ void __launch_bounds__(256) window_stats_kernel(const __nv_bfloat16* 
 #pragma unroll
     for (int s = 8; s; s >>= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
     if (lane == 0) {
-      out[r] = i < rows ? -1.4426950408889634f * p.lse[((int64_t)b * p.H + head) * p.Tq + i] : -INFINITY;
-      out[64 + r] = i < rows ? -t : 0.f;
+      const float lse = i < rows ? p.lse[((int64_t)b * p.H + head) * p.Tq + i] : 0.f;
+      out[r] = i < rows ? -1.4426950408889634f * lse : -INFINITY;
+      out[64 + r] = -t;
+      adds[at + r] = three_parts(-lse / p.scale);
+      adds[at + 64 + r] = three_parts(-t);
     }
   }
 }
@@ -190,10 +210,10 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
   }
 
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sX = base;                   // X0, X1
-  uint8_t* sY = base + 2 * L::kXBytes;  // [stage] Y0, Y1
-  float* sStat = reinterpret_cast<float*>(base + L::kCore);  // [stage][2][64]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(base + L::kCore + YS * L::kStatBytes);
+  uint8_t* sAdd = base;                 // keys' side: [stage] addends, zeros; then ones, zeros
+  uint8_t* sX = base + L::kAdds;        // X0, X1
+  uint8_t* sY = sX + 2 * L::kXBytes;    // [stage] Y0, Y1
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + L::kCore);
   uint64_t* x_full = bars;
   uint64_t* y_full = x_full + 1;    // [YS]
   uint64_t* y_empty = y_full + YS;  // [YS]
@@ -221,6 +241,14 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
     tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
   }
+  if (kKeys) {  // rows (1, 1, 1, 0, ..) and the zeros behind every block
+    for (int e = tid; e < kAddBytes / 16; e += L::kThreads) {
+      reinterpret_cast<uint4*>(sAdd + YS * 2 * kAddBytes)[e] = make_uint4(0x3f803f80u, 0x3f80u, 0u, 0u);
+#pragma unroll
+      for (int j = 0; j <= YS; ++j) reinterpret_cast<uint4*>(sAdd + (2 * j + 1) * kAddBytes)[e] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -247,13 +275,13 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
       uint8_t* dst = sY + st * L::kStage;
       if (lane == 0) {
         uint64_t* bar = clear ? tail : &y_full[st];
-        mbar_arrive_expect_tx(bar, L::kStage + (kKeys ? L::kStatBytes : 0));
+        mbar_arrive_expect_tx(bar, L::kStage + (kKeys ? kAddBytes : 0));
         for (int c = 0; c < DP / 64; ++c) {
           tma_load_4d(dst + c * (kY * 128), &tm_y0, bar, 64 * c, hd, y0, b);
           tma_load_4d(dst + L::kYBytes + c * (kY * 128), &tm_y1, bar, 64 * c, hd, y0, b);
         }
         if (kKeys)
-          bulk_load(sStat + st * 128, p.stat + (((int64_t)b * w.H + hd) * p.stat_tiles + y0 / kY) * 128, L::kStatBytes, bar);
+          bulk_load(sAdd + st * 2 * kAddBytes, p.adds + (((int64_t)b * w.H + hd) * p.stat_tiles + y0 / kY) * 128, kAddBytes, bar);
       }
       if (clear) {
         if (!all_lanes(mbar_wait(tail, tails & 1, abort_flag, status))) break;
@@ -288,6 +316,9 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
         const uint32_t tS = tm + 128 * bf;
         if (issuer) {
           const uint64_t x = smem_desc_sw128(sX), y = smem_desc_sw128(sY + st * L::kStage);
+          if (kKeys)  // -lse / scale into every row of S, -Delta into every row of dP
+            tc_mma_f16(tS, smem_desc_rows16(sAdd + YS * 2 * kAddBytes, kAddBytes),
+                       smem_desc_rows16(sAdd + st * 2 * kAddBytes, kAddBytes), make_idesc(1, kX, 2 * kY), 0u);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {  // S, dP
 #pragma unroll
@@ -295,7 +326,7 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
               const uint64_t yk = y + i * (L::kYBytes >> 4) + (k / 4) * (kY * 128 >> 4) + 2 * (k % 4);
               if (kKeys)
                 tc_mma_f16(tS + 64 * i, x + i * (L::kXBytes >> 4) + (k / 4) * (kX * 128 >> 4) + 2 * (k % 4), yk, idesc_s,
-                           k > 0 ? 1u : 0u);
+                           1u);
               else
                 tc_mma_f16_ts(tS + 64 * i, tm + L::kXCol + DP / 2 * i + 8 * k, yk, idesc_s, k > 0 ? 1u : 0u);
             }
@@ -343,12 +374,11 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
     const float c = w.scale * 1.4426950408889634f;
     const float2 c2 = make_float2(c, c);
     const int rlo = x0 + quarter * 32, rhi = rlo + 31;
-    // -lse and -Delta, of the row (queries' side, in the first two places) or of four columns
-    float4 nl4 = make_float4(0.f, 0.f, 0.f, 0.f), nd4 = nl4;
+    float2 nl = make_float2(0.f, 0.f), nd = nl;  // queries' side: the row's -lse and -Delta
     if (!kKeys) {
       const float* st = p.stat + (((int64_t)b * w.H + head0) * p.stat_tiles + r / kY) * 128 + r % kY;
       const bool have = r < p.stat_tiles * kY;
-      nl4.x = nl4.y = have ? __ldg(st) : -INFINITY, nd4.x = nd4.y = have ? __ldg(st + 64) : 0.f;
+      nl.x = nl.y = have ? __ldg(st) : -INFINITY, nd.x = nd.y = have ? __ldg(st + 64) : 0.f;
     }
     bool ok = true;
     if (!kKeys && set < 2) {  // set 0 brings Q's rows into tensor memory, set 1 dO's
@@ -373,16 +403,13 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
     }
     for (int t = bf; t < items; t += NB) {
       step_to(it, t, t == bf ? begin + bf : NB);
-      const int st = t % YS, y0 = it.y * kY;
-      // keys' side: the columns' statistics arrive with the tile
-      if (kKeys && !(ok = mbar_wait(&y_full[st], (t / YS) & 1, abort_flag, status))) break;
+      const int y0 = it.y * kY;
       if (!(ok = mbar_wait(&s_full[bf], (t / NB) & 1, abort_flag, status))) break;
       tc_fence_after();
-      const float* stat = sStat + st * 128;
       const int yc = y0 + 32 * h;
       const int qlo = kKeys ? w.offset + yc : w.offset + rlo, qhi = kKeys ? qlo + 31 : w.offset + rhi;
       const int klo = kKeys ? rlo : yc, khi = kKeys ? rhi : yc + 31;
-      uint32_t pw[16], dw[16], lw[16];  // P, dS, and what dS's rounding leaves
+      uint32_t pw[16], dw[16], lw[16];  // P, dS's upper part, and the rest of it
       const bool none = window_none(qlo, qhi, klo, khi, w.window, w.sinks);
       if (none) {
 #pragma unroll
@@ -400,20 +427,16 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
         }
 #pragma unroll
         for (int u = 0; u < 16; ++u) {
-          if (kKeys && (u & 1) == 0) {
-            nl4 = *reinterpret_cast<const float4*>(stat + 32 * h + 2 * u);
-            nd4 = *reinterpret_cast<const float4*>(stat + 64 + 32 * h + 2 * u);
-          }
-          const float2 nl = kKeys && (u & 1) ? make_float2(nl4.z, nl4.w) : make_float2(nl4.x, nl4.y);
-          const float2 nd = kKeys && (u & 1) ? make_float2(nd4.z, nd4.w) : make_float2(nd4.x, nd4.y);
-          const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * u]), __uint_as_float(s[2 * u + 1])), c2, nl);
+          const float2 s2 = make_float2(__uint_as_float(s[2 * u]), __uint_as_float(s[2 * u + 1]));
+          const float2 d2 = make_float2(__uint_as_float(d[2 * u]), __uint_as_float(d[2 * u + 1]));
+          const float2 x = kKeys ? __fmul2_rn(s2, c2) : __ffma2_rn(s2, c2, nl);
           const float2 pr = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-          const float2 e = __fadd2_rn(make_float2(__uint_as_float(d[2 * u]), __uint_as_float(d[2 * u + 1])), nd);
+          const float2 e = kKeys ? d2 : __fadd2_rn(d2, nd);
           const float2 ds = __fmul2_rn(pr, e);
           pw[u] = pack2<__nv_bfloat16>(pr.x, pr.y);
-          dw[u] = pack2<__nv_bfloat16>(ds.x, ds.y);
-          const float2 hi = unpack2<__nv_bfloat16>(dw[u]);
-          lw[u] = pack2<__nv_bfloat16>(ds.x - hi.x, ds.y - hi.y);
+          const uint32_t dx = __float_as_uint(ds.x), dy = __float_as_uint(ds.y);
+          dw[u] = __byte_perm(dx, dy, 0x7632);  // the upper halves: dS cut to bf16
+          lw[u] = pack2<__nv_bfloat16>(ds.x - __uint_as_float(dx & 0xffff0000u), ds.y - __uint_as_float(dy & 0xffff0000u));
         }
         if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {  // clear what is hidden, whatever it came to
 #pragma unroll
@@ -515,7 +538,7 @@ WindowParams window_params(const NoiseWindow* a, int* status);
 
 struct WindowPlan {
   int q_tiles, k_tiles, sink_tiles, sink_splits, splits, slots;  // slots: partial sums per (sequence, key head)
-  int64_t stat_bytes, bytes;
+  int64_t stat_bytes, add_bytes, bytes;
 };
 
 // How the keys' side is split: items (a 64-query tile of one head) per CTA at most `chunk`, the share that gives
@@ -538,7 +561,8 @@ static WindowPlan window_plan(const NoiseWindow* a) {
   p.sink_splits = p.sink_tiles > 0 && sink_items > sink_chunk + sink_chunk / 2 ? (int)((sink_items + sink_chunk - 1) / sink_chunk) : 1;
   p.slots = (p.sink_splits > 1 ? p.sink_tiles * p.sink_splits : 0) + (p.splits > 1 ? (int)plain * p.splits : 0);
   p.stat_bytes = ((int64_t)a->B * a->H * p.q_tiles * 512 + 255) / 256 * 256;
-  p.bytes = p.stat_bytes + (int64_t)a->B * a->Hk * p.slots * 2 * 128 * a->D * 4;
+  p.add_bytes = (int64_t)a->B * a->H * p.q_tiles * kAddBytes;
+  p.bytes = p.stat_bytes + p.add_bytes + (int64_t)a->B * a->Hk * p.slots * 2 * 128 * a->D * 4;
   return p;
 }
 
@@ -566,7 +590,8 @@ static int launch_window_backward(const NoiseWindow* a, const void* dout, const 
   LaunchScope scope(kKindAttention, s, 2 + (plan.sink_splits > 1) + (plan.splits > 1));
   window_stats_kernel<<<dim3(plan.q_tiles, a->H, a->B), 256, 0, s>>>(
       reinterpret_cast<const __nv_bfloat16*>(a->out), reinterpret_cast<const __nv_bfloat16*>(dout), a->B > 1 ? ds[0] : 0,
-      a->Tq > 1 ? ds[1] : 0, a->H > 1 ? ds[2] : 0, g.w, const_cast<float*>(g.stat));
+      a->Tq > 1 ? ds[1] : 0, a->H > 1 ? ds[2] : 0, g.w, const_cast<float*>(g.stat),
+      const_cast<uint4*>(g.adds));
   window_backward_kernel<DP><<<(unsigned)(key_ctas + query_ctas), L::kThreads, L::kSmem, s>>>(m, g, (int)key_ctas);
   const int join = 64;
   if (plan.sink_splits > 1)
@@ -605,7 +630,8 @@ extern "C" int noise_window_attention_backward(const NoiseWindow* a, const void*
   WindowGrad g{};
   g.w = window_params(a, status);
   g.stat = reinterpret_cast<const float*>(workspace), g.stat_tiles = plan.q_tiles;
-  g.partial = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + plan.stat_bytes);
+  uint8_t* at = reinterpret_cast<uint8_t*>(workspace) + plan.stat_bytes;
+  g.adds = reinterpret_cast<const uint4*>(at), g.partial = reinterpret_cast<float*>(at + plan.add_bytes);
   g.dq = dq, g.dk = dk, g.dv = dv;
   g.q = reinterpret_cast<const __nv_bfloat16*>(a->q), g.dout = reinterpret_cast<const __nv_bfloat16*>(dout);
   const int64_t size[3] = {a->B, a->Tq, a->H};
