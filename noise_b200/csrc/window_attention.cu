@@ -277,10 +277,7 @@ __global__ void __launch_bounds__(WinFwd<DP>::kThreads, WinFwd<DP>::kCtas)
       for (int t = 0; t < walk.n; ++t) {
         const int kt = walk.tile(t);
         if (!needs(g, kt)) continue;
-        if (!mbar_wait(&s_full[g], n & 1, abort_flag, status)) {
-          ok = false;
-          break;
-        }
+        if (!(ok = mbar_wait_warp(&s_full[g], n & 1, abort_flag, status))) break;
         tc_fence_after();
         const int k0 = kt * KT;
         // P of the tile, with m as it stands; `raise` (for the whole warp) first lifts m to the rows' maxima
@@ -357,7 +354,7 @@ __global__ void __launch_bounds__(WinFwd<DP>::kThreads, WinFwd<DP>::kCtas)
         if (lane == 0) mbar_arrive(&p_full[g]);
         ++n;
       }
-      if (ok && mbar_wait(&o_full[g], 0, abort_flag, status)) {
+      if (ok && mbar_wait_warp(&o_full[g], 0, abort_flag, status)) {
         tc_fence_after();
         const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         const bool have = i < rows;

@@ -404,7 +404,7 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
     for (int t = bf; t < items; t += NB) {
       step_to(it, t, t == bf ? begin + bf : NB);
       const int y0 = it.y * kY;
-      if (!(ok = mbar_wait(&s_full[bf], (t / NB) & 1, abort_flag, status))) break;
+      if (!(ok = mbar_wait_warp(&s_full[bf], (t / NB) & 1, abort_flag, status))) break;
       tc_fence_after();
       const int yc = y0 + 32 * h;
       const int qlo = kKeys ? w.offset + yc : w.offset + rlo, qhi = kKeys ? qlo + 31 : w.offset + rhi;
@@ -454,7 +454,7 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[bf]);
     }
-    if (ok && mbar_wait(done, 0, abort_flag, status)) {
+    if (ok && mbar_wait_warp(done, 0, abort_flag, status)) {
       tc_fence_after();
       const bool have = kKeys ? r < length : r < rows;
       // the gradients' 32-column chunks (keys' side: dK's, then dV's) go round the sets
