@@ -127,16 +127,25 @@ def _qk_check(q, k, rope, positions, q_weight, k_weight, order):
     return B, T, H, Hk, D, stride
 
 
-def _qk_plan(q, k, rope, positions, q_weight, k_weight, order, eps):
-    """(leading fields of NoiseQkNorm, table rows, positions' stride, steps of q, of k, of contiguous results)."""
+def _qk_plan(q, k, rope, positions, q_weight, k_weight, order, eps, dq=None, dk=None):
+    """(leading fields of NoiseQkNorm, table rows, positions' stride, steps of q, of k, of contiguous results, of dq and
+    dk, workspace bytes)."""
     eps = float(eps)
     key = ('qk', q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, rope.shape, rope.stride(), rope.dtype,
-           _meta(positions), _meta(q_weight), _meta(k_weight), order, eps)
+           _meta(positions), _meta(q_weight), _meta(k_weight), order, eps, _meta(dq), _meta(dk))
 
     def make():
         B, T, H, Hk, D, stride = _qk_check(q, k, rope, positions, q_weight, k_weight, order)
         head = (DTYPE_CODES[q.dtype], ORDERS[order], B, T, H, Hk, D, eps)
-        return head, len(rope), stride, _steps(q, True), _steps(k, True), (T * H * D, H * D, D, T * Hk * D, Hk * D, D)
+        grad_steps, need = (None, None), 0
+        if dq is not None:
+            if dq.shape != q.shape or dk.shape != k.shape or dq.dtype != q.dtype or dk.dtype != q.dtype:
+                raise ValueError('qk_norm_rope_backward: dq and dk must have the shapes and type of q and k')
+            grad_steps = _steps(dq, True), _steps(dk, True)
+            if q_weight is not None or k_weight is not None:
+                need = int(_lib.load().noise_qk_norm_workspace_bytes(D))
+        return (head, len(rope), stride, _steps(q, True), _steps(k, True),
+                (T * H * D, H * D, D, T * Hk * D, Hk * D, D), *grad_steps, need)
 
     plan = checked(key, make)
     if rope.data_ptr() & 15:
@@ -157,7 +166,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, *, positi
     t row t), and a position outside the table gives NaN rows. q_weight, k_weight: fp32 [D] weights of the
     norms. out: (q_out, k_out) to write to, of any addressable layout (a cache's rows, or q and k themselves).
     Returns (q_out, k_out)."""
-    head, table, stride, qs, ks, out_steps = _qk_plan(q, k, rope, positions, q_weight, k_weight, order, eps)
+    head, table, stride, qs, ks, out_steps, *_ = _qk_plan(q, k, rope, positions, q_weight, k_weight, order, eps)
     if out is None:
         q_out, k_out = _like(q), _like(k)
     else:
@@ -182,18 +191,15 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     """Gradients of qk_norm_rope: dq, dk are those of its results, q, k and the rest its inputs. Returns the
     gradients of (q, k, q_weight, k_weight); a weight that was not given has None. The weights' sums run in a
     fixed order."""
-    head, table, stride, qs, ks, out_steps = _qk_plan(q, k, rope, positions, q_weight, k_weight, order, eps)
-    if dq.shape != q.shape or dk.shape != k.shape or dq.dtype != q.dtype or dk.dtype != q.dtype:
-        raise ValueError('qk_norm_rope_backward: dq and dk must have the shapes and type of q and k')
+    head, table, stride, qs, ks, out_steps, dqs, dks, need = _qk_plan(q, k, rope, positions, q_weight, k_weight, order, eps,
+                                                                      dq, dk)
     device = device_index('qk_norm_rope_backward', q, k, dq, dk, rope, positions, q_weight, k_weight)
     (q, qs), (k, ks) = _rows(q, qs, True), _rows(k, ks, True)
-    (dq, dqs), (dk, dks) = _rows(dq, _steps(dq, True), True), _rows(dk, _steps(dk, True), True)
+    (dq, dqs), (dk, dks) = _rows(dq, dqs, True), _rows(dk, dks, True)
     gq, gk = _like(q), _like(k)
-    gwq, gwk = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
-    ws, need = None, 0
-    if gwq is not None or gwk is not None:
-        need = int(_lib.load().noise_qk_norm_workspace_bytes(q.shape[3]))
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    gwq = None if q_weight is None else torch.empty_like(q_weight)
+    gwk = None if k_weight is None else torch.empty_like(k_weight)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     a = _lib.QK_NORM.pack(*head, rope.data_ptr(), table, _pointer(positions), stride, _pointer(q_weight),
                           _pointer(k_weight), q.data_ptr(), k.data_ptr(), dq.data_ptr(), dk.data_ptr(), gq.data_ptr(),
                           gk.data_ptr(), *qs, *ks, *dqs, *dks, *out_steps, _pointer(gwq), _pointer(gwk))
@@ -263,16 +269,24 @@ def _window_check(name, q, k, v, window, sinks, lengths, offset, scale, token):
     return DTYPE_CODES[q.dtype], B, Tq, Tk, H, Hk, D, offset, window, sinks, scale
 
 
-def _window_plan(name, q, k, v, window, sinks, lengths, offset, scale, token):
-    """(leading fields of NoiseWindow, steps of q, k, v)."""
+def _window_plan(name, q, k, v, window, sinks, lengths, offset, scale, token, dout=None, out=None, lse=None):
+    """(leading fields of NoiseWindow, steps of q, k, v, of dout)."""
     window, offset = (n if n is None else int(n) for n in (window, offset))
     sinks, scale = int(sinks), scale if scale is None else float(scale)
     key = (name, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, _meta(lengths),
-           window, sinks, offset, scale)
+           window, sinks, offset, scale, _meta(dout), _meta(out), _meta(lse))
 
     def make():
         head = _window_check(name, q, k, v, window, sinks, lengths, offset, scale, token)
-        return head, _steps(q.unsqueeze(1) if token else q, False), _steps(k, False), _steps(v, False)
+        if dout is not None:
+            if q.dtype != torch.bfloat16:
+                raise ValueError(f'{name}: bf16 only, got {q.dtype}')
+            if dout.shape != q.shape or out.shape != q.shape or dout.dtype != q.dtype or out.dtype != q.dtype:
+                raise ValueError(f'{name}: dout and out must have the shape and type of q')
+            if lse.shape != (head[1], head[4], head[2]) or lse.dtype != torch.float32:
+                raise ValueError(f'{name}: lse must be fp32 [B, H, Tq], got {lse.dtype} {tuple(lse.shape)}')
+        return (head, _steps(q.unsqueeze(1) if token else q, False), _steps(k, False), _steps(v, False),
+                None if dout is None else _steps(dout, False))
 
     return checked(key, make)
 
@@ -289,7 +303,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     status: an int32 word that a device wait which ran out sets; without one the call waits for the
     GPU and checks its own. Returns (out [B, Tq, H, D], lse fp32 [B, H, Tq])."""
     name = 'window_attention'
-    head, qs, ks, vs = _window_plan(name, q, k, v, window, sinks, lengths, offset, scale, False)
+    head, qs, ks, vs, _ = _window_plan(name, q, k, v, window, sinks, lengths, offset, scale, False)
     st = _Status(name, status)
     device = device_index(name, q, k, v, lengths)
     out = _like(q)
@@ -311,19 +325,13 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     """Gradients of window_attention (bf16): dout is out's, and out, lse are what it returned for the same
     arguments. Padding rows get zeros. Sums run in a fixed order. Returns (dq, dk, dv)."""
     name = 'window_attention_backward'
-    head, qs, ks, vs = _window_plan(name, q, k, v, window, sinks, lengths, offset, scale, False)
-    if q.dtype != torch.bfloat16:
-        raise ValueError(f'{name}: bf16 only, got {q.dtype}')
-    if dout.shape != q.shape or out.shape != q.shape or dout.dtype != q.dtype or out.dtype != q.dtype:
-        raise ValueError(f'{name}: dout and out must have the shape and type of q')
-    if lse.shape != (head[1], head[4], head[2]) or lse.dtype != torch.float32:
-        raise ValueError(f'{name}: lse must be fp32 [B, H, Tq], got {lse.dtype} {tuple(lse.shape)}')
+    head, qs, ks, vs, gs = _window_plan(name, q, k, v, window, sinks, lengths, offset, scale, False, dout, out, lse)
     st = _Status(name, status)
     device = device_index(name, q, k, v, dout, out, lse, lengths)
     if not q.numel():
         return torch.empty_like(q), torch.zeros_like(k), torch.zeros_like(v)
     dq, dk, dv = _like(q), _like(k), _like(v)
-    (q, qs), (k, ks), (v, vs), (dout, gs) = _rows(q, qs), _rows(k, ks), _rows(v, vs), _rows(dout, _steps(dout, False))
+    (q, qs), (k, ks), (v, vs), (dout, gs) = _rows(q, qs), _rows(k, ks), _rows(v, vs), _rows(dout, gs)
     out, lse = out.contiguous(), lse.contiguous()
     if out.data_ptr() & 15:
         out = out.clone()
@@ -345,7 +353,7 @@ def window_attention_token(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, le
     name = 'window_attention_token'
     if lengths is None:
         raise ValueError(f'{name}: lengths are required')
-    head, qs, ks, vs = _window_plan(name, q, k, v, window, sinks, lengths, None, scale, True)
+    head, qs, ks, vs, _ = _window_plan(name, q, k, v, window, sinks, lengths, None, scale, True)
     device = device_index(name, q, k, v, lengths)
     out = _like(q)
     if not out.numel():

@@ -16,12 +16,17 @@ from .attention import DTYPE_CODES, _meta, _pointer, checked, device_index, laun
 MAX_ENTRIES = 1024
 
 
-def _matrix(t: torch.Tensor):
-    """A matrix whose columns are contiguous and whose rows do not overlap (t, or a copy), and its row stride."""
+def _row_stride(t: torch.Tensor):
+    """Row stride of a matrix whose columns are contiguous and whose rows do not overlap, else None."""
     rows, cols = t.shape
     if (t.stride(1) != 1 and cols != 1) or (t.stride(0) < cols and rows != 1):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.stride(0) if rows > 1 else cols
+        return None
+    return t.stride(0) if rows > 1 else cols
+
+
+def _matrix(t: torch.Tensor, stride):
+    """t, or a contiguous copy where its layout cannot be taken, and its row stride."""
+    return (t, stride) if stride is not None else (t.clone(memory_format=torch.contiguous_format), t.shape[1])
 
 
 def _check(name, logits, ids, teacher, temperature, softcap, dloss, lse, fused):
@@ -45,13 +50,15 @@ def _check(name, logits, ids, teacher, temperature, softcap, dloss, lse, fused):
         if V > limit:
             raise ValueError(f'{name}: loss and gradient in one pass take at most {limit} logits a row of {logits.dtype}, '
                              f'got {V}; use distill_loss and distill_backward')
-    return DTYPE_CODES[logits.dtype], DTYPE_CODES[teacher.dtype], ids.dtype == torch.int64, V, ids.shape[1]
+    return ((DTYPE_CODES[logits.dtype], DTYPE_CODES[teacher.dtype], ids.dtype == torch.int64, V, ids.shape[1]),
+            _row_stride(logits), _row_stride(ids), _row_stride(teacher))
 
 
 def _call(name, logits, ids, teacher, temperature, softcap, dloss=None, lse=None, want_loss=True, want_grad=False):
     temperature, softcap = float(temperature), float(softcap)
     key = (name, _meta(logits), _meta(ids), _meta(teacher), temperature, softcap, _meta(dloss), _meta(lse))
-    head = checked(key, lambda: _check(name, logits, ids, teacher, temperature, softcap, dloss, lse, want_loss and want_grad))
+    head, ld, ids_ld, teacher_ld = checked(
+        key, lambda: _check(name, logits, ids, teacher, temperature, softcap, dloss, lse, want_loss and want_grad))
     N, V = logits.shape
     device = device_index(name, logits, ids, teacher, dloss, lse)
     where = logits.device
@@ -59,7 +66,8 @@ def _call(name, logits, ids, teacher, temperature, softcap, dloss=None, lse=None
     out_lse = torch.empty(N, dtype=torch.float64, device=where) if want_loss and not want_grad else None
     grad = torch.empty(N, V, dtype=logits.dtype, device=where) if want_grad else None
     if N:
-        (logits, ld), (ids, ids_ld), (teacher, teacher_ld) = _matrix(logits), _matrix(ids), _matrix(teacher)
+        (logits, ld), (ids, ids_ld) = _matrix(logits, ld), _matrix(ids, ids_ld)
+        teacher, teacher_ld = _matrix(teacher, teacher_ld)
         dloss = None if dloss is None else dloss.contiguous()
         lse = None if lse is None else lse.contiguous()
         a = _lib.DISTILL.pack(*head, temperature, softcap, N, ld, ids_ld, teacher_ld, V, logits.data_ptr(),
