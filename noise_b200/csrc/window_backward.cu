@@ -50,9 +50,9 @@ struct WindowGrad {
   int64_t q_step[3], dout_step[3];
 };
 
-// Boxes of 128 rows for a CTA's own tiles, of 64 for the streamed ones.
+// Boxes of 128 rows for the keys' side's own tiles, of 64 for the streamed ones.
 struct WindowMaps {
-  CUtensorMap k128, v128, q64, o64, q128, o128, k64, v64;
+  CUtensorMap k128, v128, q64, o64, k64, v64;
 };
 
 // The addends of S and dP: rows of eight bf16, 64 rows each.
@@ -127,10 +127,10 @@ __global__ void __launch_bounds__(256) window_stats_kernel(const __nv_bfloat16* 
 
 // One CTA of either side; `index` is its place in that side's order.
 template <int DP, bool kKeys>
-__device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUtensorMap& tm_x1, const CUtensorMap& tm_y0,
-                                            const CUtensorMap& tm_y1, const WindowGrad& p, int index) {
+__device__ __forceinline__ void window_side(const WindowMaps& m, const WindowGrad& p, int index) {
   using L = WinBwd<DP>;
   constexpr int NB = L::NB, YS = L::YS, kX = L::kX, kY = L::kY;
+  const CUtensorMap &tm_y0 = kKeys ? m.q64 : m.k64, &tm_y1 = kKeys ? m.o64 : m.v64;
   extern __shared__ uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const WindowParams& w = p.w;
@@ -232,8 +232,7 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbarrier_init();
-    prefetch_tensormap(&tm_x0);
-    prefetch_tensormap(&tm_x1);
+    if (kKeys) prefetch_tensormap(&m.k128), prefetch_tensormap(&m.v128);
     prefetch_tensormap(&tm_y0);
     prefetch_tensormap(&tm_y1);
   }
@@ -260,8 +259,8 @@ __device__ __forceinline__ void window_side(const CUtensorMap& tm_x0, const CUte
     if (kKeys && lane == 0) {
       mbar_arrive_expect_tx(x_full, 2 * L::kXBytes);
       for (int c = 0; c < DP / 64; ++c) {
-        tma_load_4d(sX + c * (kX * 128), &tm_x0, x_full, 64 * c, head, x0, b);
-        tma_load_4d(sX + L::kXBytes + c * (kX * 128), &tm_x1, x_full, 64 * c, head, x0, b);
+        tma_load_4d(sX + c * (kX * 128), &m.k128, x_full, 64 * c, head, x0, b);
+        tma_load_4d(sX + L::kXBytes + c * (kX * 128), &m.v128, x_full, 64 * c, head, x0, b);
       }
     }
     const int end = kKeys ? rows : length, total = kKeys ? w.Tq : w.Tk;
@@ -503,9 +502,9 @@ template <int DP>
 __global__ void __launch_bounds__(WinBwd<DP>::kThreads, WinBwd<DP>::kCtas)
     window_backward_kernel(const __grid_constant__ WindowMaps m, const __grid_constant__ WindowGrad p, int key_ctas) {
   if ((int)blockIdx.x < key_ctas)
-    window_side<DP, true>(m.k128, m.v128, m.q64, m.o64, p, blockIdx.x);
+    window_side<DP, true>(m, p, blockIdx.x);
   else
-    window_side<DP, false>(m.q128, m.o128, m.k64, m.v64, p, blockIdx.x - key_ctas);
+    window_side<DP, false>(m, p, blockIdx.x - key_ctas);
 }
 
 // dK and dV of split key tiles: their partial sums added in order. One thread per four columns.
@@ -578,7 +577,6 @@ static int launch_window_backward(const NoiseWindow* a, const void* dout, const 
   };
   if (map(&m.k128, a->k, a->Tk, a->Hk, a->k_stride, L::kX) || map(&m.v128, a->v, a->Tk, a->Hk, a->v_stride, L::kX) ||
       map(&m.q64, a->q, a->Tq, a->H, a->q_stride, L::kY) || map(&m.o64, dout, a->Tq, a->H, ds, L::kY) ||
-      map(&m.q128, a->q, a->Tq, a->H, a->q_stride, L::kX) || map(&m.o128, dout, a->Tq, a->H, ds, L::kX) ||
       map(&m.k64, a->k, a->Tk, a->Hk, a->k_stride, L::kY) || map(&m.v64, a->v, a->Tk, a->Hk, a->v_stride, L::kY))
     return kStatusBadArgument;
   const int plain = plan.k_tiles - plan.sink_tiles;
