@@ -15,6 +15,13 @@
 // lane and the mean is a shuffle over the row's lanes. A lane takes several heads of one token at a
 // time: their loads are in flight together and share the table's values. Query and key rows go to
 // different CTAs of one launch, so that the weight gradients need one accumulator set a thread.
+//
+// Measured: 8 + 8 heads of 64 in 16,384 tokens of a packed bf16 projection: 16.4 us, 4.1 TB/s. 12 + 4 heads of 96 in
+// 22,662 tokens with weights: forward 33 us, 4.2 TB/s, gradient 58 us, 3.6 TB/s, and 6 us for the weights' sums. Next to
+// HBM stand the instructions (120 a lane and row forward, 206 in the gradient; 60 % of the issue slots) and their
+// latency at 32 warps an SM. Eight values of either half a lane save instructions and cost registers: 97 against 60 us for
+// the gradient; copies through a ring in shared memory, 68 against 58; arithmetic without pairs, 24 instructions more,
+// the same time.
 #include "operators.cuh"
 #include "profile.cuh"
 #include "ptx.cuh"

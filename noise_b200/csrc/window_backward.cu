@@ -13,20 +13,26 @@
 // and make the result depend on timing.
 //
 // The sides have one body. X0, X1 are the CTA's own 128-row tiles, Y0, Y1 the streamed 64-row tiles:
-//   S  = X0 Y0^T, dP = X1 Y1^T  (both operands in shared memory, accumulators in tensor memory)
+//   S  = X0 Y0^T, dP = X1 Y1^T  (X in shared memory on the keys' side, in tensor memory, where its product is faster,
+//                                on the queries' side, which has columns left; accumulators in tensor memory)
 //   P and dS, as 16-bit pairs over the columns that S and dP lay in, are the A operands of
 //   keys' side (X = K, V; Y = Q, dO; rows are keys):     dV += P Y1, dK += dS Y0
 //   queries' side (X = Q, dO; Y = K, V; rows are queries): dQ += dS Y0
-// with Y0, Y1 read a second time, now as MN-major B operands, from the same shared memory. On the keys' side lse and Delta
-// belong to columns: one more product, of a row of ones with their three bf16 parts (24 bits), puts -lse / scale under S
-// and -Delta under dP. Read from shared memory by every thread instead they took turns with the tensor core's own reads:
-// 240 us against 217 for both sides at 8 x 2,048 tokens, 8 heads of 64, window 1,024. What bounds the kernel is
-// each item's chain (S and dP, the warps' arithmetic, the gradients' products), not a unit, so two items are in
-// flight per SM (two CTAs with one buffer of S and dP each at a head width of 64, one CTA with two buffers at 128)
-// and eight warps share an item, each with 32 rows and half of the columns.
+// with Y0, Y1 read a second time, now as MN-major B operands, from the same shared memory. On the keys' side lse and
+// Delta belong to columns: one more product, of rows of ones with their three bf16 parts (24 bits), puts -lse / scale
+// under S and -Delta under dP. Read from shared memory by every thread instead they took turns with the tensor core's
+// own reads: 240 us against 217.
+//
+// Measured (all launches) at B 8, T 2048, 8 heads of 64, window 1024, 4 sinks: 217 us, 298 TFLOP/s of the five products
+// over the visible pairs; at 4 padded sequences of up to 1,999 tokens, 12 heads on 4 of 128, window 511, 16 sinks:
+// 110 us. What bounds it is each item's chain (S and dP, the warps' arithmetic, the gradients' products) at 64, the
+// products' rate and a CTA's first and last item at 128. So two items are in flight per SM (two CTAs with one buffer of
+// S and dP each at 64, one CTA with two buffers at 128) and eight warps share an item, each with 32 rows and half of
+// the columns. One persistent CTA an SM with P and dS beside S and dP: 197 and 125 against 211 and 100 us.
 // P is rounded to bf16, as the tensor core needs. dS goes in as two bf16 numbers, its upper half (cut, which costs one
-// permute a pair) and the rest rounded, 16 bits in all (the columns that dP lay in hold both): rounded to one, dQ and dK were off by 2.4e-3 of their norm where the rounding of
-// the result alone makes 1.7e-3. Sums are fp32.
+// permute a pair; rounded, 235 against 227 us) and the rest rounded, 16 bits in all, in the columns that dP lay in:
+// rounded to one, dQ and dK were off by 2.4e-3 of their norm where the rounding of the result alone makes 1.7e-3, and
+// the kernel took 20 us less. Sums are fp32.
 //
 // Sinks are seen by every later query, so their key tiles have far more work than the others: it is dealt in
 // chunks to several CTAs that write fp32 partial sums, added in order by a last launch. Grouped heads with few
