@@ -203,3 +203,43 @@ def test_distill_error_of_a_capture():
     x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + oo.EPS32)
     # tf32 products keep 10 bits of either operand: 2^-10 relative in all
     assert rel(reassemble(cap, 'lm_head', err), full.T @ x) <= 2e-3
+
+
+def test_repeated_calls_look_at_each_tensor():
+    """Checks are kept by shapes and strides; addresses and devices are each call's own. The attention calls copy an
+    operand they cannot load from, so the results are the same bits. The distillation takes any address of an fp32, but
+    the address decides which of a row's 99 logits a thread adds up: two orders of a sum of n positive fp32 terms differ
+    by at most 2 n 2^-24 of it. So lse and with it the loss may differ by 2 * 99 * 2^-24, and by the roundings of the
+    entries' sum (5 terms below 32, up to 4 roundings each: 20 * 32 * 2^-24); a gradient, at most 1, by 2 * 99 * 2^-24
+    and its own roundings (8 * 2^-24)."""
+    from noise_b200.attention import qk_norm_rope, qk_norm_rope_backward, window_attention, window_attention_token
+    from noise_b200.distill import distill_loss_grad
+    g = torch.Generator().manual_seed(5)
+
+    def odd(t):  # the same values, shape and strides at an address that the kernels cannot load from
+        flat = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view(t.shape)
+
+    q, k, v = (torch.randn(2, 40, n, 64, generator=g).bfloat16().cuda() for n in (4, 2, 2))
+    rope = torch.randn(40, 64, generator=g).cuda()
+    lengths = torch.tensor([40, 17], dtype=torch.int32, device='cuda')
+    ids = torch.randint(0, 99, (8, 5), generator=g).int().cuda()
+    z, teacher = torch.randn(8, 99, generator=g).cuda(), torch.randn(8, 5, generator=g).cuda()
+    calls = [(lambda q, k, v: qk_norm_rope(q, k, rope), (q, k, v)),
+             (lambda q, k, v: qk_norm_rope_backward(q, k, q, k, rope)[:2], (q, k, v)),
+             (lambda q, k, v: window_attention(q, k, v, 9, 1, lengths=lengths), (q, k, v)),
+             (lambda q, k, v: (window_attention_token(q, k, v, lengths, 9, 1),), (q[:, 0].contiguous(), k, v)),
+             (lambda z, i, t: distill_loss_grad(z, i, t), (z, ids, teacher))]
+    for call, args in calls:
+        want = call(*args)
+        for moved in (args, tuple(odd(t) for t in args), args):
+            for a, b in zip(want, call(*moved)):
+                if args[0] is z and moved is not args:
+                    assert (a - b).abs().max() <= (2 * 99 + (640 if a.dim() == 1 else 8)) * 2.0 ** -24
+                else:
+                    assert torch.equal(a, b)
+        with pytest.raises(ValueError, match='one CUDA device'):
+            call(args[0], args[1].cpu(), args[2])
+    with pytest.raises(ValueError, match='aligned'):
+        qk_norm_rope(q, k, odd(rope))

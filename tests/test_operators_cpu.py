@@ -76,6 +76,8 @@ ONE = torch.ones(2, dtype=torch.int32)
     ((z(2, 5, 4, 64), z(2, 5, 2, 64), z(2, 5, 2, 64), 3, -2), {}, 'negative'),
     ((z(2, 5, 4, 64), z(2, 5, 2, 64), z(2, 5, 2, 64), 3), dict(scale=0.0), 'scale'),
     ((z(2, 5, 4, 64), z(2, 5, 2, 64), z(2, 5, 2, 64), 3), dict(scale=float('nan')), 'scale'),
+    ((z(2, 5, 4, 64), z(2, 5, 2, 64), z(2, 5, 2, 64), 3), dict(scale=2.0 ** -101), 'scale'),
+    ((z(2, 5, 4, 64), z(2, 5, 2, 64), z(2, 5, 2, 64), 3), dict(scale=2.0 ** 101), 'scale'),
     ((z(2, 5, 4, 64), z(2, 5, 2, 64), z(2, 5, 2, 64), 3), dict(offset=1), 'offset'),
     ((z(2, 5, 4, 64), z(2, 5, 2, 64), z(2, 5, 2, 64), 3), dict(lengths=ONE.long()), 'lengths'),
     ((z(2, 5, 4, 64), z(2, 5, 2, 64), z(2, 5, 2, 64), 3), dict(lengths=torch.ones(3, dtype=torch.int32)), 'lengths'),

@@ -127,6 +127,19 @@ def test_backward(case):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize('D,factor,window,sinks', [(64, 8, 100, 3), (128, 8, 400, 0), (64, 2.0 ** -40, 50, 1)])
+def test_backward_of_large_and_tiny_scores(D, factor, window, sinks):
+    """-lse / scale and -Delta go through the tensor core on the keys' side: scores of up to a few hundred keep their
+    differences (their sums' error is deltas' term in Z, |lse| being at most Z + log Tk), and vanishing ones their size."""
+    from noise_b200.attention import window_attention, window_attention_backward
+    g = torch.Generator().manual_seed(D + window)
+    q, k, v, do = (randn(g, 1, 333, n, D, dtype=torch.bfloat16) for n in (2, 1, 1, 2))
+    q = q * factor
+    c = [t.cuda() for t in (q, k, v, do)]
+    out, lse = window_attention(*c[:3], window, sinks)
+    check_backward(window_attention_backward(c[3], *c[:3], out, lse, window, sinks), do, q, k, v, window, sinks, None, None)
+
+
 def test_oracle_gradient_matches_differences():
     """The float64 formulas that the kernel is held to, against central differences of the float64 forward."""
     g = torch.Generator().manual_seed(31)
