@@ -24,7 +24,8 @@
 //
 // The K entries are handled apart from the dense pass: every column is first written as if no entry
 // named it, then the thread of an id's first entry rewrites that column with the sum over the entries
-// of the same id, in entry order. Repeated ids are therefore added in the same order every time.
+// of the same id, in entry order. Repeated ids are therefore added in the same order every time. Which entries repeat
+// is found by a vote of a warp up to 32 entries and by a table of the ids beyond.
 #include "operators.cuh"
 #include "profile.cuh"
 #include "ptx.cuh"
@@ -61,6 +62,7 @@ struct DistillParams {
   int64_t grad_ld;
   int64_t rows;
   int V, K, parts;       // parts: CTAs per row
+  int table;             // places of the table of ids, a power of two of at least 2 K
   float tau, cap;
 };
 
@@ -420,24 +422,48 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
     __syncthreads();  // the dense stores of this CTA come before its entries' stores
     finish();
     const int e0 = begin * N - phase, e1 = min(p.V, end * N - phase);
-    for (int k = tid; k - lane < p.K; k += kDsThreads) {  // whole warps: equal ids among 32 entries by a vote
-      const int id = k < p.K ? s_id[k] : -1;
-      const uint32_t equal = __match_any_sync(0xffffffffu, id);
-      if (id < e0 || id >= e1 || id < 0) continue;
-      bool first = (equal & ((1u << lane) - 1u)) == 0, again = (equal >> lane) > 1u;
-#pragma unroll 8
-      for (int i = 0; i < p.K; ++i) {
-        if (p.K <= 32) break;
-        first = first && !(s_id[i] == id && i < k);
-        again = again || (s_id[i] == id && i > k);
-      }
-      if (!first) continue;
+    auto here = [&](int id) { return id >= e0 && id < e1 && id >= 0; };
+    auto rewrite = [&](int k, int id, bool again) {
       int other;
       float pj = exp2f(((k == tid ? t0 : entry(k, other)) - top) * t_scale) * inv_mass;
       if (again)
         for (int i = k + 1; i < p.K; ++i)
           if (s_id[i] == id) pj += exp2f((entry(i, other) - top) * t_scale) * inv_mass;
       g[id] = from_f32<E>(slope(value1(k == tid ? z_id : to_f32(z[id])), pj));
+    };
+    if (p.K <= 32) {  // equal ids by a vote of one warp
+      if (warp == 0) {
+        const int id = lane < p.K ? s_id[lane] : -1;
+        const uint32_t equal = __match_any_sync(0xffffffffu, id);
+        if (here(id) && (equal & ((1u << lane) - 1u)) == 0) rewrite(lane, id, (equal >> lane) > 1u);
+      }
+    } else {
+      // by a table of the ids, over the memory that the row has left: a place's id (its sign bit: named again), its
+      // first entry, and each entry's place. Where an id lies depends on timing; what the table says of it does not.
+      int* t_id = reinterpret_cast<int*>(hold);
+      int* t_first = t_id + p.table;
+      uint16_t* at = reinterpret_cast<uint16_t*>(t_first + p.table);
+      for (int i = tid; i < p.table; i += kDsThreads) t_id[i] = -1, t_first[i] = kDsMaxK;
+      __syncthreads();
+      for (int k = tid; k < p.K; k += kDsThreads) {
+        const int id = s_id[k];
+        if (!here(id)) continue;
+        uint32_t h = (uint32_t)id * 2654435769u >> 16;  // the multiplier of Fibonacci hashing, 2^32 / golden ratio
+        while (true) {  // at most half of the places are taken
+          h &= p.table - 1;
+          const int was = atomicCAS(&t_id[h], -1, id);
+          if (was == -1 || was == id) break;
+          ++h;
+        }
+        atomicMin(&t_first[h], k);
+        at[k] = (uint16_t)h;
+      }
+      __syncthreads();
+      for (int k = tid; k < p.K; k += kDsThreads)
+        if (here(s_id[k]) && t_first[at[k]] != k) t_id[at[k]] = s_id[k] | (int)0x80000000;
+      __syncthreads();
+      for (int k = tid; k < p.K; k += kDsThreads)
+        if (here(s_id[k]) && t_first[at[k]] == k) rewrite(k, s_id[k], t_id[at[k]] < 0);
     }
   } else {
     __syncthreads();
@@ -470,6 +496,11 @@ static int launch_distill(DistillParams& p, cudaStream_t s) {
     const int64_t need = ds_hold_bytes(p.V, sizeof(E), kCap == kCapBound, parts);
     if (need > kDsRowBytes) return kStatusUnsupported;
     smem = (int)need;
+  }
+  if (kMode != kDsLoss && p.K > 32) {
+    for (p.table = 64; p.table < 2 * p.K;) p.table *= 2;
+    const int need = p.table * 8 + (p.K * 2 + 15) / 16 * 16;  // at most 18 KB
+    smem = smem > need ? smem : need;
   }
   if (p.rows * parts > INT32_MAX) return kStatusUnsupported;
   p.parts = parts;
