@@ -97,20 +97,28 @@ __device__ __forceinline__ uint4 slot_pack(const float2 (&v)[DsSlot<E>::kN / 2])
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 ex2_pair(float2 x) { return make_float2(ex2_approx(x.x), ex2_approx(x.y)); }
 
-// tanh to about 2 ulp. Away from 0 from e = exp(-2 |x|): (1 - e) / (1 + e). Near 0, where 1 - e would cancel, from a
-// polynomial x + x^3 Q(x^2), |x| <= 0.55: Q is a least-squares fit of degree 4 at Chebyshev nodes, off by 4e-9 of tanh.
-__device__ __forceinline__ float ds_tanh(float x) {
-  const float a = fabsf(x), u = x * x;
-  const float e = ex2_approx(a * -2.8853900817779268f);
-  const float far = (1.f - e) * rcp_approx(1.f + e);
-  float q = fmaf(-0.006615746766f, u, 0.0213127397f);
-  q = fmaf(q, u, -0.05391006544f);
-  q = fmaf(q, u, 0.1333311796f);
-  q = fmaf(q, u, -0.3333333135f);
-  const float near = fmaf(x * u, q, x);
-  return a < 0.55f ? near : copysignf(far, x);
+// tanh to about 2 ulp. Up to |x| = 1 from a polynomial x + x^3 Q(x^2): Q is a least-squares fit of degree 6 at Chebyshev
+// nodes, off by 6e-9 of tanh. Beyond, where 1 - e no longer cancels, from e = exp(-2 |x|): (1 - e) / (1 + e). Logits
+// within the soft cap, nearly all of a trained model's, so take no special function for their tanh.
+__device__ __forceinline__ float2 tanh_near(float2 x) {
+  const float2 u = __fmul2_rn(x, x);
+  float2 q = __ffma2_rn(both(-3.552270937e-4f), u, both(2.289985307e-3f));
+  q = __ffma2_rn(q, u, both(-7.930326276e-3f));
+  q = __ffma2_rn(q, u, both(2.147581428e-2f));
+  q = __ffma2_rn(q, u, both(-5.387599394e-2f));
+  q = __ffma2_rn(q, u, both(1.333228201e-1f));
+  q = __ffma2_rn(q, u, both(-3.333329260e-1f));
+  return __ffma2_rn(__fmul2_rn(x, u), q, x);
 }
-__device__ __forceinline__ float2 ds_tanh(float2 x) { return make_float2(ds_tanh(x.x), ds_tanh(x.y)); }
+__device__ __forceinline__ float tanh_far(float x) {
+  const float e = ex2_approx(fabsf(x) * -2.8853900817779268f);
+  return copysignf((1.f - e) * rcp_approx(1.f + e), x);
+}
+__device__ __forceinline__ float2 ds_tanh(float2 x) {
+  const float2 near = tanh_near(x);
+  return make_float2(fabsf(x.x) <= 1.f ? near.x : tanh_far(x.x), fabsf(x.y) <= 1.f ? near.y : tanh_far(x.y));
+}
+__device__ __forceinline__ float ds_tanh(float x) { return ds_tanh(both(x)).x; }
 
 // A reference m and the sum of 2^(scale (. - m)); an empty or all -inf set is (-inf, 0). The difference is taken
 // before the scale, so that values near the type's lowest do not turn into -inf.
@@ -192,7 +200,19 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
     }
   };
   start();
-  auto value = [&](float2 x) { return kCap ? ds_tanh(__fmul2_rn(x, both(inv_cap))) : x; };
+  auto values = [&](float2 (&v)[N / 2]) {  // of a slot; the same numbers on either way
+    if (!kCap) return;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) v[i] = __fmul2_rn(v[i], both(inv_cap)), top = max3(top, fabsf(v[i].x), fabsf(v[i].y));
+    if (top <= 1.f) {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) v[i] = tanh_near(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) v[i] = ds_tanh(v[i]);
+    }
+  };
   auto value1 = [&](float x) { return kCap ? ds_tanh(x * inv_cap) : x; };
 
   // Entry k: its id (-1: absent) and logit. A thread keeps its first one, k = tid, in registers from the start.
@@ -210,6 +230,27 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
   int id0 = -1;
   float t0 = -INFINITY;
   if (tid < p.K) t0 = entry(tid, id0);
+  // the teacher's maximum and mass: p_k = 2^(t_scale (t_k - max)) / mass, 0 for absent entries. The warps' parts of them
+  // are formed here, while the row's first copies are on their way.
+  const float t_scale = inv_tau * kLog2e;
+  if (warp * 32 < p.K) {
+    MaxSum c{t0, t0 == -INFINITY ? 0.f : 1.f};
+    if (tid < p.K) s_id[tid] = id0;
+    for (int k = tid + kDsThreads; k < p.K; k += kDsThreads) {
+      int id;
+      const float t = entry(k, id);
+      s_id[k] = id;
+      c.join(t, t == -INFINITY ? 0.f : 1.f, t_scale);
+    }
+    float top = c.m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float mass = c.m == -INFINITY ? c.s : c.s * exp2f((c.m - top) * t_scale);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+    if (lane == 0) red[2][warp] = top, red[3][warp] = mass;
+  }
+  const float z_id = id0 >= 0 ? to_f32(z[id0]) : 0.f;
 
   MaxSum a{kBound ? scale : -INFINITY, 0.f};
   if constexpr (kMode != kDsGrad) {
@@ -217,10 +258,11 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
     auto add = [&](const uint4& w, int slot, float2& sum) {
       float2 v[N / 2];
       slot_values<E>(w, v);
+      values(v);
       if constexpr (kBound) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-          const float2 th = value(v[i]);
+          const float2 th = v[i];
           const float2 e = ex2_pair(__ffma2_rn(th, both(scale), both(-scale)));
           sum = __fadd2_rn(sum, e);
           if (kHold) v[i] = __fmul2_rn(e, __ffma2_rn(make_float2(-th.x, -th.y), th, both(1.f)));
@@ -234,7 +276,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
       } else {
         const float2 off = both(a.m == -INFINITY ? 0.f : -a.m);
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) sum = __fadd2_rn(sum, ex2_pair(__ffma2_rn(value(v[i]), both(scale), off)));
+        for (int i = 0; i < N / 2; ++i) sum = __fadd2_rn(sum, ex2_pair(__ffma2_rn(v[i], both(scale), off)));
       }
     };
     // a reference that the slots from `slot` on, `count` of them, do not overflow
@@ -268,31 +310,16 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
       else a.join(x, x == -INFINITY ? 0.f : 1.f);
     });
   }
-  // the teacher's maximum and mass: p_k = 2^(t_scale (t_k - max)) / mass, 0 for absent entries
-  const float t_scale = inv_tau * kLog2e;
-  MaxSum c{t0, t0 == -INFINITY ? 0.f : 1.f};
-  if (tid < p.K) s_id[tid] = id0;
-  for (int k = tid + kDsThreads; k < p.K; k += kDsThreads) {
-    int id;
-    const float t = entry(k, id);
-    s_id[k] = id;
-    c.join(t, t == -INFINITY ? 0.f : 1.f, t_scale);
-  }
-  const float z_id = id0 >= 0 ? to_f32(z[id0]) : 0.f;
-
-  // one sweep for the row's sum and the teacher's
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    if (kMode != kDsGrad) {
-      const float os = __shfl_xor_sync(0xffffffffu, a.s, o);
-      if (kBound) a.s += os;
-      else a.join(__shfl_xor_sync(0xffffffffu, a.m, o), os);
-    }
-    if (warp * 32 < p.K) c.join(__shfl_xor_sync(0xffffffffu, c.m, o), __shfl_xor_sync(0xffffffffu, c.s, o), t_scale);
+    if (kMode == kDsGrad) break;
+    const float os = __shfl_xor_sync(0xffffffffu, a.s, o);
+    if (kBound) a.s += os;
+    else a.join(__shfl_xor_sync(0xffffffffu, a.m, o), os);
   }
-  if (lane == 0) red[0][warp] = a.m, red[1][warp] = a.s, red[2][warp] = c.m, red[3][warp] = c.s;
+  if (lane == 0) red[0][warp] = a.m, red[1][warp] = a.s;
   __syncthreads();
-  c = MaxSum{red[2][0], red[3][0]};
+  MaxSum c{red[2][0], red[3][0]};
 #pragma unroll
   for (int w = 1; w < kDsWarps; ++w)
     if (w * 32 < p.K) c.join(red[2][w], red[3][w], t_scale);
@@ -396,9 +423,10 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
         }
       } else {
         slot_values<E>(w, v);
+        values(v);
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-          const float2 x = value(v[i]);
+          const float2 x = v[i];
           float2 y = __ffma2_rn(x, both(scale), both(-ref));
           if (kMode == kDsGrad) y = __fadd2_rn(y, both(-low));
           v[i] = __fmul2_rn(ex2_pair(y), gain);
