@@ -61,9 +61,9 @@ struct DistillParams {
   void* grad;
   int64_t grad_ld;
   int64_t rows;
-  int V, K, parts;       // parts: CTAs per row
+  int V, K, parts, shift;  // parts: CTAs per row, 2^shift
   int table;             // places of the table of ids, a power of two of at least 2 K
-  float tau, cap;
+  float tau, cap, inv_tau, inv_cap;
 };
 
 // A slot is 16 bytes of a row, counted from the 16-byte boundary at or before its first element, so the
@@ -144,15 +144,15 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
   __shared__ float red[5][kDsWarps];
   __shared__ float2 part;  // this CTA's (m, s), read by the cluster
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x / p.parts;
-  const int rank = blockIdx.x - (int)(row * p.parts);
+  const int64_t row = blockIdx.x >> p.shift;
+  const int rank = blockIdx.x & (p.parts - 1);
   const E* z = reinterpret_cast<const E*>(p.logits) + row * p.ld;
   const int phase = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(E));
   const E* z0 = z - phase;  // 16-byte aligned; element e of the row is z0[e + phase]
   const int slots = (p.V + phase + N - 1) / N;
-  const int share = (slots + p.parts - 1) / p.parts;
+  const int share = (slots + p.parts - 1) >> p.shift;
   const int begin = min(slots, rank * share), end = min(slots, begin + share);
-  const float inv_tau = 1.0f / p.tau, inv_cap = kCap ? 1.0f / p.cap : 0.f;
+  const float inv_tau = p.inv_tau, inv_cap = p.inv_cap;
   // s in base 2 is scale * v, with v = z, or tanh(z / c)
   const float scale = (kCap ? p.cap : 1.f) * inv_tau * kLog2e;
 
@@ -171,32 +171,41 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
   };
   const uint4* z16 = reinterpret_cast<const uint4*>(z0);
   // f(batch of slots, its first slot, how many) for this thread's slots first + tid, + kDsThreads, ..: each thread
-  // copies its own slots into its own places, kDsAhead batches ahead
-  auto place = [&](int batch, int u, int slot) {
-    return kHold ? slot - begin : ((batch % kDsAhead) * kDsBatch + u) * kDsThreads + tid;
+  // copies its own slots into its own places, kDsAhead batches ahead, on a ring or (kHold) to where they stay
+  constexpr uint32_t kPitch = kDsThreads * 16, kBatchBytes = kDsBatch * kPitch, kWrap = kHold ? 0u : kDsAhead * kBatchBytes;
+  const uint32_t own = (kHold ? first - begin : 0) * 16 + tid * 16;
+  const uint4* source = z16 + first + tid;
+  int coming = last - first - tid;  // slots from this thread's next one on
+  uint32_t into = own;
+  auto advance = [&](uint32_t& at) {
+    at += kBatchBytes;
+    if (!kHold && at >= kWrap) at -= kWrap;
   };
-  auto issue = [&](int batch) {
+  const uint32_t hold0 = smem_u32(hold);
+  auto issue = [&] {
 #pragma unroll
-    for (int u = 0; u < kDsBatch; ++u) {
-      const int slot = first + tid + (batch * kDsBatch + u) * kDsThreads;
-      if (slot < last) cp_async16(smem_u32(hold + place(batch, u, slot)), z16 + slot);
-    }
+    for (int u = 0; u < kDsBatch; ++u)
+      if (u * kDsThreads < coming) cp_async16(hold0 + into + u * kPitch, source + u * kDsThreads);
     cp_async_commit();
+    source += kDsBatch * kDsThreads, coming -= kDsBatch * kDsThreads;
+    advance(into);
   };
   auto start = [&] {
 #pragma unroll
-    for (int i = 0; i < kDsAhead - 1; ++i) issue(i);
+    for (int i = 0; i < kDsAhead - 1; ++i) issue();
   };
   auto sweep = [&](auto&& f) {
-    int batch = 0;
-    for (int slot = first + tid; slot < last; slot += kDsBatch * kDsThreads, ++batch) {
-      issue(batch + kDsAhead - 1);
+    uint32_t from = own;
+    for (int slot = first + tid; slot < last; slot += kDsBatch * kDsThreads) {
+      issue();
       cp_async_wait<kDsAhead - 1>();
       uint4 w[kDsBatch];
+      const int count = min(kDsBatch, (last - slot + kDsThreads - 1) / kDsThreads);
 #pragma unroll
       for (int u = 0; u < kDsBatch; ++u)
-        if (slot + u * kDsThreads < last) w[u] = hold[place(batch, u, slot + u * kDsThreads)];
-      f(w, slot, min(kDsBatch, (last - slot + kDsThreads - 1) / kDsThreads));
+        if (u < count) w[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(hold) + from + u * kPitch);
+      advance(from);
+      f(w, slot, count);
     }
   };
   start();
@@ -347,7 +356,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
   }
 
   // the loss's terms, added up behind the dense gradient
-  if (kMode != kDsGrad && rank == 0) {
+  if (kMode != kDsGrad && rank == 0 && warp * 32 < p.K) {
     const float log_mass = logf(mass), log_sum = log2f(a.s);
     float l = 0.f;
     auto term = [&](int id, float t, float x) {
@@ -370,7 +379,8 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
     if (kMode == kDsGrad || rank != 0 || tid != 0) return;
     float l = red[4][0];
 #pragma unroll
-    for (int w = 1; w < kDsWarps; ++w) l += red[4][w];
+    for (int w = 1; w < kDsWarps; ++w)
+      if (w * 32 < p.K) l += red[4][w];
     p.loss[row] = empty ? 0.f : p.tau * p.tau * l;
     // in 64 bits: the gradient's exponentials have the error of this number in common
     if (p.lse) p.lse[row] = 0.6931471805599453094 * ((double)a.m + log2((double)a.s));
@@ -532,6 +542,8 @@ static int launch_distill(DistillParams& p, cudaStream_t s) {
   }
   if (p.rows * parts > INT32_MAX) return kStatusUnsupported;
   p.parts = parts;
+  for (p.shift = 0; 1 << p.shift < parts;) ++p.shift;
+  p.inv_tau = 1.0f / p.tau, p.inv_cap = kCap ? 1.0f / p.cap : 0.f;
   if (!opt_in(distill_kernel<E, kMode, kCap>, kMode == kDsBoth ? kDsRowBytes : kDsRing)) return kStatusLaunchFailed;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
