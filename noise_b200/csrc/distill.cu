@@ -7,17 +7,17 @@
 //   d loss / dz_j = tau (exp(s_j - lse) - sum over k with id_k = j of p_k) (1 - tanh^2(z_j / c))
 // An entry whose id is outside [0, V) is absent; a row without an entry above -inf has loss and gradient 0.
 //
-// Bound: HBM, with the special-function unit (16 results a cycle and SM) next: a soft-capped logit takes three
-// (the exponential and reciprocal of its tanh, the exponential of s). The loss reads a row once. Loss and gradient
+// Bound: HBM, with the issue slots and the special-function unit (16 results a cycle and SM) next: a logit takes
+// one of it, one beyond the soft cap three. The loss reads a row once. Loss and gradient
 // together read it once and write it once; the row waits between the two halves in shared memory:
 //   - with a soft cap s <= c / tau, so that is the sums' reference, no maximum is sought, and what waits is
 //     exp(s - c / tau) (1 - tanh^2), which the second half only multiplies by one factor of the row;
 //   - without one a thread takes the maximum of its first values as its reference and looks for another only
 //     when a sum leaves fp32's safe range; what waits are the loaded words, and their exponential is taken again.
-// What it takes is bytes in flight: a CTA is 128 threads, eight to an SM, and each thread copies its own 16-byte
-// slots into shared memory six batches ahead (with loads to registers, 137 instead of 111 us for 16,384 rows of 4,096
-// soft-capped fp32 logits with 32 entries, loss and gradient; CTAs of 256 threads 180). That is 4.9 TB/s; 2,047 rows of
-// 50,257 bf16 logits take 131 us for the loss and then the gradient from its lse, 4.7 TB/s.
+// What it takes is bytes in flight and few instructions beside: a CTA is 128 threads, eight to an SM, and each thread
+// copies its own 16-byte slots into shared memory some batches ahead (loads to registers instead: a quarter more time;
+// CTAs of 256 threads 45 % more, of 64 10 %). Loss and gradient of 16,384 rows of 4,096 soft-capped fp32 logits with 32
+// entries: 99 us, 5.4 TB/s; 2,047 rows of 50,257 bf16 logits, the loss and then the gradient from its lse: 131 us, 4.7 TB/s.
 //
 // A row too long for one CTA, or one of a few rows, is spread over a cluster of up to 8 CTAs whose sums meet
 // through distributed shared memory, so no second launch or workspace is needed.
@@ -37,8 +37,14 @@ constexpr int kDsResident = 8;           // CTAs an SM holds
 constexpr int kDsMaxK = 1024;
 constexpr int kDsMaxCluster = 8;
 constexpr int kDsRowBytes = 192 * 1024;  // shared memory that holds a CTA's part of a row, at most
-constexpr int kDsBatch = 2, kDsAhead = 6;  // slots of a batch; batches a thread has in flight
-constexpr int kDsRing = kDsAhead * kDsBatch * kDsThreads * 16;
+// Slots of a batch, and batches a thread has in flight: on a ring, or as deep as it pays where the row stays. (Six batches
+// of two everywhere: the gradient alone of 16,384 rows of 4,096 took 125 us instead of 100.)
+template <bool kHold>
+struct DsFlow {
+  static constexpr int kBatch = kHold ? 1 : 2, kAhead = kHold ? 8 : 3;
+};
+constexpr int kDsTable = 2 * kDsMaxK * 8 + kDsMaxK * 2;  // the table of ids, at most
+constexpr int kDsRing = DsFlow<false>::kAhead * DsFlow<false>::kBatch * kDsThreads * 16;
 
 enum : int { kDsLoss = 0, kDsGrad = 1, kDsBoth = 2 };
 // No soft cap; one whose c / tau bounds every exponential within fp32 (2 c / tau <= 80); any other.
@@ -137,6 +143,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
   constexpr int N = DsSlot<E>::kN;
   constexpr bool kHold = kMode == kDsBoth;  // the row stays in shared memory
   constexpr bool kBound = kCap == kCapBound;
+  constexpr int kDsBatch = DsFlow<kHold>::kBatch, kDsAhead = DsFlow<kHold>::kAhead;
   constexpr float kLog2e = 1.4426950408889634f;
   // the row's slots (kHold; with a bound soft cap N / 4 planes of fp32 per slot), or a ring of batches in flight
   extern __shared__ uint4 hold[];
@@ -522,12 +529,12 @@ static int64_t ds_hold_bytes(int V, int elem, bool planes, int parts) {
 template <typename E, int kMode, int kCap>
 static int launch_distill(DistillParams& p, cudaStream_t s) {
   static KernelOptIn opt_in;
-  // CTAs per row: until every SM has two, of at least two batches a thread; more where a row must fit shared memory.
+  // CTAs per row: until every SM has two, of at least four slots a thread; more where a row must fit shared memory.
   // (Splitting 2,047 rows of 50,257 over clusters of 4 to even out the last CTAs took 188 us instead of 139.)
   const int64_t slots = ((int64_t)p.V + DsSlot<E>::kN - 1) / DsSlot<E>::kN;
   const int64_t want = 2 * (int64_t)device_sm_count();
   int parts = 1;
-  while (parts < kDsMaxCluster && p.rows * parts < want && slots / (2 * parts) >= 2 * kDsBatch * kDsThreads) parts *= 2;
+  while (parts < kDsMaxCluster && p.rows * parts < want && slots / (2 * parts) >= 4 * kDsThreads) parts *= 2;
   int smem = kDsRing;
   if (kMode == kDsBoth) {
     while (parts < kDsMaxCluster && ds_hold_bytes(p.V, sizeof(E), kCap == kCapBound, parts) > kDsRowBytes / 4) parts *= 2;
@@ -537,14 +544,14 @@ static int launch_distill(DistillParams& p, cudaStream_t s) {
   }
   if (kMode != kDsLoss && p.K > 32) {
     for (p.table = 64; p.table < 2 * p.K;) p.table *= 2;
-    const int need = p.table * 8 + (p.K * 2 + 15) / 16 * 16;  // at most 18 KB
+    const int need = p.table * 8 + (p.K * 2 + 15) / 16 * 16;
     smem = smem > need ? smem : need;
   }
   if (p.rows * parts > INT32_MAX) return kStatusUnsupported;
   p.parts = parts;
   for (p.shift = 0; 1 << p.shift < parts;) ++p.shift;
   p.inv_tau = 1.0f / p.tau, p.inv_cap = kCap ? 1.0f / p.cap : 0.f;
-  if (!opt_in(distill_kernel<E, kMode, kCap>, kMode == kDsBoth ? kDsRowBytes : kDsRing)) return kStatusLaunchFailed;
+  if (!opt_in(distill_kernel<E, kMode, kCap>, kMode == kDsBoth ? kDsRowBytes : kDsRing > kDsTable ? kDsRing : kDsTable)) return kStatusLaunchFailed;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = (unsigned)parts, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;

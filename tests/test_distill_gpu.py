@@ -99,6 +99,34 @@ def test_loss_and_gradient(case):
         assert dev[0].isfinite().all() or case[0] > 4  # the view was only read
 
 
+@pytest.mark.parametrize('N,V,K', [(2, 200003, 180), (400, 3001, 90)])
+def test_entries_that_repeat_or_meet_in_the_table(N, V, K):
+    """More than 32 entries: ids that all fall on one place of the table of ids, each named twice and far apart; one id
+    that every entry names; ids that follow one another. Twice, with equal bits."""
+    from noise_b200.distill import distill_backward, distill_loss, distill_loss_grad
+    places = 64
+    while places < 2 * K:
+        places *= 2
+    every = torch.arange(V)
+    place = ((every * 2654435769) % 2 ** 32 >> 16) % places
+    few = every[place == place.bincount().argmax()][:K // 2]
+    g = torch.Generator().manual_seed(K)
+    z, t = torch.randn(N, V, generator=g).mul_(3), torch.randn(N, K, generator=g)
+    ids = torch.randint(0, V, (N, K), generator=g)
+    ids[0] = torch.cat([few, few, every[:K]])[:K]
+    ids[1] = 77
+    if N > 2:
+        ids[2] = every[100:100 + K]
+    up = torch.rand(N, generator=g)
+    dev = [x.cuda() for x in (z, ids.int(), t)]
+    loss, lse = distill_loss(*dev)
+    want, q, p, slope, E = expected(z, ids, t, 1.0, 0.0)
+    for call in (lambda: distill_loss_grad(*dev, dloss=up.cuda())[1], lambda: distill_backward(up.cuda(), *dev, lse)):
+        got = call()
+        check_grad(got, up, q, p, slope, E, 1.0, z.dtype)
+        assert torch.equal(got, call())
+
+
 def test_gradient_matches_differences():
     """Central differences of the float64 loss: truncation h^2 ~ 1e-8, so 1e-6 holds beside the kernel's fp32."""
     from noise_b200.distill import distill_loss_grad
