@@ -163,19 +163,16 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
   // s in base 2 is scale * v, with v = z, or tanh(z / c)
   const float scale = (kCap ? p.cap : 1.f) * inv_tau * kLog2e;
 
-  // This CTA's whole slots, and its share of the row's at most two partial ones: one element after the other, by
-  // the first thread.
+  // This CTA's whole slots, and its share of the row's at most two partial ones, an element a thread: the head's by the
+  // first warp, the tail's by the second.
   const int head = (N - phase) % N, tail = head + (p.V - head > 0 ? (p.V - head) / N * N : 0);  // [head, tail): whole slots
   const int skip = phase ? 1 : 0;
   const int first = max(begin, skip), last = min(end, skip + (tail - head) / N);
   const bool has_head = phase && begin == 0 && end > 0, has_tail = tail < p.V && end == slots && end > begin;
-  auto edges = [&](auto&& f) {
-    if (tid != 0) return;
-    if (has_head)
-      for (int e = 0; e < min(head, p.V); ++e) f(e);
-    if (has_tail)
-      for (int e = max(tail, head); e < p.V; ++e) f(e);
-  };
+  int edge = -1;
+  if (has_head && tid < min(head, p.V)) edge = tid;
+  if (has_tail && tid >= 32 && tid - 32 < p.V - max(tail, head)) edge = max(tail, head) + tid - 32;
+  const float z_edge = edge >= 0 ? to_f32(z[edge]) : 0.f;
   const uint4* z16 = reinterpret_cast<const uint4*>(z0);
   // f(batch of slots, its first slot, how many) for this thread's slots first + tid, + kDsThreads, ..: each thread
   // copies its own slots into its own places, kDsAhead batches ahead, on a ring or (kHold) to where they stay
@@ -320,11 +317,11 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
       a.s += sum.x + sum.y;
     };
     sweep(take);
-    edges([&](int e) {
-      const float x = value1(to_f32(z[e])) * scale;
+    if (edge >= 0) {
+      const float x = value1(z_edge) * scale;
       if (kBound) a.s += ex2_approx(x - scale);
       else a.join(x, x == -INFINITY ? 0.f : 1.f);
-    });
+    }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -424,7 +421,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) v[i] = both(0.f);
       for (int slot = first + tid; slot < last; slot += kDsThreads) write(slot, v);
-      edges([&](int e) { g[e] = from_f32<E>(0.f); });
+      if (edge >= 0) g[edge] = from_f32<E>(0.f);
       __syncthreads();
       finish();
       return;
@@ -463,7 +460,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
       for (int slot = first + tid; slot < last; slot += kDsThreads)
         spread(kBound ? make_uint4(0u, 0u, 0u, 0u) : hold[slot - begin], slot);
     }
-    edges([&](int e) { g[e] = from_f32<E>(slope(value1(to_f32(z[e])), 0.f)); });
+    if (edge >= 0) g[edge] = from_f32<E>(slope(value1(z_edge), 0.f));
     __syncthreads();  // the dense stores of this CTA come before its entries' stores
     finish();
     const int e0 = begin * N - phase, e1 = min(p.V, end * N - phase);
