@@ -32,9 +32,9 @@
 
 namespace noise {
 
-constexpr int kDsThreads = 128, kDsWarps = kDsThreads / 32;
-constexpr int kDsResident = 8;           // CTAs an SM holds
+constexpr int kDsSmThreads = 1024;       // threads an SM holds, in CTAs of 128 or 32
 constexpr int kDsMaxK = 1024;
+constexpr int kDsSmallSlots = 512;       // 16-byte slots of a row that one warp takes
 constexpr int kDsMaxCluster = 8;
 constexpr int kDsRowBytes = 192 * 1024;  // shared memory that holds a CTA's part of a row, at most
 // Slots of a batch, and batches a thread has in flight: on a ring, or as deep as it pays where the row stays. (Six batches
@@ -42,9 +42,9 @@ constexpr int kDsRowBytes = 192 * 1024;  // shared memory that holds a CTA's par
 template <bool kHold>
 struct DsFlow {
   static constexpr int kBatch = kHold ? 1 : 2, kAhead = kHold ? 8 : 3;
+  static constexpr int ring(int threads) { return kHold ? 0 : kAhead * kBatch * threads * 16; }
 };
 constexpr int kDsTable = 2 * kDsMaxK * 8 + kDsMaxK * 2;  // the table of ids, at most
-constexpr int kDsRing = DsFlow<false>::kAhead * DsFlow<false>::kBatch * kDsThreads * 16;
 
 enum : int { kDsLoss = 0, kDsGrad = 1, kDsBoth = 2 };
 // No soft cap; one whose c / tau bounds every exponential within fp32 (2 c / tau <= 80); any other.
@@ -68,6 +68,7 @@ struct DistillParams {
   int64_t grad_ld;
   int64_t rows;
   int V, K, parts, shift;  // parts: CTAs per row, 2^shift
+  int id_at;             // bytes of dynamic shared memory before the entries' ids
   int table;             // places of the table of ids, a power of two of at least 2 K
   float tau, cap, inv_tau, inv_cap;
 };
@@ -138,8 +139,8 @@ struct MaxSum {
   }
 };
 
-template <typename E, int kMode, int kCap>
-__global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const __grid_constant__ DistillParams p) {
+template <typename E, int kMode, int kCap, int kDsThreads>
+__global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill_kernel(const __grid_constant__ DistillParams p) {
   constexpr int N = DsSlot<E>::kN;
   constexpr bool kHold = kMode == kDsBoth;  // the row stays in shared memory
   constexpr bool kBound = kCap == kCapBound;
@@ -147,7 +148,8 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
   constexpr float kLog2e = 1.4426950408889634f;
   // the row's slots (kHold; with a bound soft cap N / 4 planes of fp32 per slot), or a ring of batches in flight
   extern __shared__ uint4 hold[];
-  __shared__ __align__(16) int s_id[kDsMaxK];
+  int* s_id = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(hold) + p.id_at);  // [K]
+  constexpr int kDsWarps = kDsThreads / 32;
   __shared__ float red[5][kDsWarps];
   __shared__ float2 part;  // this CTA's (m, s), read by the cluster
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -163,15 +165,15 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
   // s in base 2 is scale * v, with v = z, or tanh(z / c)
   const float scale = (kCap ? p.cap : 1.f) * inv_tau * kLog2e;
 
-  // This CTA's whole slots, and its share of the row's at most two partial ones, an element a thread: the head's by the
-  // first warp, the tail's by the second.
+  // This CTA's whole slots, and its share of the row's at most two partial ones, an element a thread: the head's by
+  // threads 0 .. 6, the tail's by threads 8 .. 14.
   const int head = (N - phase) % N, tail = head + (p.V - head > 0 ? (p.V - head) / N * N : 0);  // [head, tail): whole slots
   const int skip = phase ? 1 : 0;
   const int first = max(begin, skip), last = min(end, skip + (tail - head) / N);
   const bool has_head = phase && begin == 0 && end > 0, has_tail = tail < p.V && end == slots && end > begin;
   int edge = -1;
   if (has_head && tid < min(head, p.V)) edge = tid;
-  if (has_tail && tid >= 32 && tid - 32 < p.V - max(tail, head)) edge = max(tail, head) + tid - 32;
+  if (has_tail && tid >= 8 && tid - 8 < p.V - max(tail, head)) edge = max(tail, head) + tid - 8;
   const float z_edge = edge >= 0 ? to_f32(z[edge]) : 0.f;
   const uint4* z16 = reinterpret_cast<const uint4*>(z0);
   // f(batch of slots, its first slot, how many) for this thread's slots first + tid, + kDsThreads, ..: each thread
@@ -248,11 +250,11 @@ __global__ void __launch_bounds__(kDsThreads, kDsResident) distill_kernel(const 
   const float t_scale = inv_tau * kLog2e;
   if (warp * 32 < p.K) {
     MaxSum c{t0, t0 == -INFINITY ? 0.f : 1.f};
-    if (tid < p.K) s_id[tid] = id0;
+    if (kMode != kDsLoss && tid < p.K) s_id[tid] = id0;
     for (int k = tid + kDsThreads; k < p.K; k += kDsThreads) {
       int id;
       const float t = entry(k, id);
-      s_id[k] = id;
+      if (kMode != kDsLoss) s_id[k] = id;
       c.join(t, t == -INFINITY ? 0.f : 1.f, t_scale);
     }
     float top = c.m;
@@ -523,45 +525,54 @@ static int64_t ds_hold_bytes(int V, int elem, bool planes, int parts) {
   return share * (planes ? 4 * n : 16);
 }
 
+template <typename E, int kMode, int kCap, int kThreads>
+static int launch_distill(DistillParams& p, int parts, int smem, cudaStream_t s) {
+  static KernelOptIn opt_in;
+  constexpr int kMost = (kMode == kDsBoth ? kDsRowBytes : kDsTable) + kDsMaxK * 4;
+  if (!opt_in(distill_kernel<E, kMode, kCap, kThreads>, kMost)) return kStatusLaunchFailed;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)parts, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.rows * parts)), cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (size_t)smem, cfg.stream = s;
+  cfg.attrs = &attr, cfg.numAttrs = kMode != kDsGrad && parts > 1;  // the gradient's CTAs share nothing
+  LaunchScope scope(kKindLoss, s);
+  if (cudaLaunchKernelEx(&cfg, distill_kernel<E, kMode, kCap, kThreads>, p) != cudaSuccess) {
+    cudaGetLastError();
+    return kStatusLaunchFailed;
+  }
+  return kStatusOk;
+}
+
 template <typename E, int kMode, int kCap>
 static int launch_distill(DistillParams& p, cudaStream_t s) {
-  static KernelOptIn opt_in;
   // CTAs per row: until every SM has two, of at least four slots a thread; more where a row must fit shared memory.
   // (Splitting 2,047 rows of 50,257 over clusters of 4 to even out the last CTAs took 188 us instead of 139.)
   const int64_t slots = ((int64_t)p.V + DsSlot<E>::kN - 1) / DsSlot<E>::kN;
   const int64_t want = 2 * (int64_t)device_sm_count();
   int parts = 1;
-  while (parts < kDsMaxCluster && p.rows * parts < want && slots / (2 * parts) >= 4 * kDsThreads) parts *= 2;
-  int smem = kDsRing;
-  if (kMode == kDsBoth) {
+  while (parts < kDsMaxCluster && p.rows * parts < want && slots / (2 * parts) >= 4 * 128) parts *= 2;
+  if (kMode == kDsBoth)
     while (parts < kDsMaxCluster && ds_hold_bytes(p.V, sizeof(E), kCap == kCapBound, parts) > kDsRowBytes / 4) parts *= 2;
-    const int64_t need = ds_hold_bytes(p.V, sizeof(E), kCap == kCapBound, parts);
-    if (need > kDsRowBytes) return kStatusUnsupported;
-    smem = (int)need;
+  // CTAs of one warp where there are more rows than fit the GPU in CTAs of four and a row is short.
+  const bool small = parts == 1 && p.rows > 8 * (int64_t)device_sm_count() && slots <= kDsSmallSlots && p.K <= 128;
+  int64_t smem = DsFlow<kMode == kDsBoth>::ring(small ? 32 : 128);
+  static_assert(DsFlow<false>::ring(128) <= kDsTable, "the opt-in covers the ring");
+  if (kMode == kDsBoth) smem = ds_hold_bytes(p.V, sizeof(E), kCap == kCapBound, parts);
+  if (smem > kDsRowBytes || p.rows * parts > INT32_MAX) return kStatusUnsupported;
+  if (kMode != kDsLoss) {
+    if (p.K > 32) {
+      for (p.table = 64; p.table < 2 * p.K;) p.table *= 2;
+      smem = max(smem, (int64_t)p.table * 8 + (p.K * 2 + 15) / 16 * 16);
+    }
+    p.id_at = (int)smem, smem += (p.K + 3) / 4 * 16;
   }
-  if (kMode != kDsLoss && p.K > 32) {
-    for (p.table = 64; p.table < 2 * p.K;) p.table *= 2;
-    const int need = p.table * 8 + (p.K * 2 + 15) / 16 * 16;
-    smem = smem > need ? smem : need;
-  }
-  if (p.rows * parts > INT32_MAX) return kStatusUnsupported;
   p.parts = parts;
   for (p.shift = 0; 1 << p.shift < parts;) ++p.shift;
   p.inv_tau = 1.0f / p.tau, p.inv_cap = kCap ? 1.0f / p.cap : 0.f;
-  if (!opt_in(distill_kernel<E, kMode, kCap>, kMode == kDsBoth ? kDsRowBytes : kDsRing > kDsTable ? kDsRing : kDsTable)) return kStatusLaunchFailed;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)parts, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.rows * parts)), cfg.blockDim = dim3(kDsThreads);
-  cfg.dynamicSmemBytes = (size_t)smem, cfg.stream = s;
-  cfg.attrs = &attr, cfg.numAttrs = kMode == kDsGrad ? 0 : 1;  // the gradient's CTAs share nothing
-  LaunchScope scope(kKindLoss, s);
-  if (cudaLaunchKernelEx(&cfg, distill_kernel<E, kMode, kCap>, p) != cudaSuccess) {
-    cudaGetLastError();
-    return kStatusLaunchFailed;
-  }
-  return kStatusOk;
+  return small ? launch_distill<E, kMode, kCap, 32>(p, parts, (int)smem, s)
+               : launch_distill<E, kMode, kCap, 128>(p, parts, (int)smem, s);
 }
 
 template <typename E, int kMode>
