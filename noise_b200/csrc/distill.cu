@@ -14,10 +14,11 @@
 //     exp(s - c / tau) (1 - tanh^2), which the second half only multiplies by one factor of the row;
 //   - without one a thread takes the maximum of its first values as its reference and looks for another only
 //     when a sum leaves fp32's safe range; what waits are the loaded words, and their exponential is taken again.
-// What it takes is bytes in flight and few instructions beside: a CTA is 128 threads, eight to an SM, and each thread
-// copies its own 16-byte slots into shared memory some batches ahead (loads to registers instead: a quarter more time;
-// CTAs of 256 threads 45 % more, of 64 10 %). Loss and gradient of 16,384 rows of 4,096 soft-capped fp32 logits with 32
-// entries: 99 us, 5.4 TB/s; 2,047 rows of 50,257 bf16 logits, the loss and then the gradient from its lse: 131 us, 4.7 TB/s.
+// What it takes is bytes in flight and few instructions beside: a CTA is 128 threads, eight to an SM (one warp where
+// rows are many and short), and each thread copies its own 16-byte slots into shared memory some batches ahead (loads to
+// registers instead: a quarter more time; CTAs of 256 threads: 45 % more). Loss and gradient of 16,384 rows of 4,096
+// soft-capped fp32 logits with 32 entries: 102 us, 5.3 TB/s; 2,047 rows of 50,257 bf16 logits, the loss and then the
+// gradient from its lse: 130 us, 4.8 TB/s.
 //
 // A row too long for one CTA, or one of a few rows, is spread over a cluster of up to 8 CTAs whose sums meet
 // through distributed shared memory, so no second launch or workspace is needed.
@@ -34,7 +35,6 @@ namespace noise {
 
 constexpr int kDsSmThreads = 1024;       // threads an SM holds, in CTAs of 128 or 32
 constexpr int kDsMaxK = 1024;
-constexpr int kDsSmallSlots = 512;       // 16-byte slots of a row that one warp takes
 constexpr int kDsMaxCluster = 8;
 constexpr int kDsRowBytes = 192 * 1024;  // shared memory that holds a CTA's part of a row, at most
 // Slots of a batch, and batches a thread has in flight: on a ring, or as deep as it pays where the row stays. (Six batches
@@ -42,6 +42,7 @@ constexpr int kDsRowBytes = 192 * 1024;  // shared memory that holds a CTA's par
 template <bool kHold>
 struct DsFlow {
   static constexpr int kBatch = kHold ? 1 : 2, kAhead = kHold ? 8 : 3;
+  static constexpr int kSmallSlots = kHold ? 512 : 1536;  // a row that one warp takes, in slots
   static constexpr int ring(int threads) { return kHold ? 0 : kAhead * kBatch * threads * 16; }
 };
 constexpr int kDsTable = 2 * kDsMaxK * 8 + kDsMaxK * 2;  // the table of ids, at most
@@ -555,8 +556,12 @@ static int launch_distill(DistillParams& p, cudaStream_t s) {
   while (parts < kDsMaxCluster && p.rows * parts < want && slots / (2 * parts) >= 4 * 128) parts *= 2;
   if (kMode == kDsBoth)
     while (parts < kDsMaxCluster && ds_hold_bytes(p.V, sizeof(E), kCap == kCapBound, parts) > kDsRowBytes / 4) parts *= 2;
-  // CTAs of one warp where there are more rows than fit the GPU in CTAs of four and a row is short.
-  const bool small = parts == 1 && p.rows > 8 * (int64_t)device_sm_count() && slots <= kDsSmallSlots && p.K <= 128;
+  // CTAs of one warp where there are more rows than fit the GPU in CTAs of four and a row is short: the steps that come
+  // once a row then wait for nothing but themselves. Loss, gradient alone and both in us, four warps against one: 9,678
+  // rows of 258 slots 51, 33, 57 / 29, 16, 37; 16,384 of 1,024 76, 98, 102 / 64, 88, 107; 6,000 of 1,251 53, 47, 70 /
+  // 43, 43, 90; 4,000 of 2,048 49, 57, 92 / 51, 59, 92. The row that stays in shared memory wants more threads a CTA.
+  const bool small = parts == 1 && p.rows > 8 * (int64_t)device_sm_count() && p.K <= 256 &&
+                     slots <= DsFlow<kMode == kDsBoth>::kSmallSlots;
   int64_t smem = DsFlow<kMode == kDsBoth>::ring(small ? 32 : 128);
   static_assert(DsFlow<false>::ring(128) <= kDsTable, "the opt-in covers the ring");
   if (kMode == kDsBoth) smem = ds_hold_bytes(p.V, sizeof(E), kCap == kCapBound, parts);

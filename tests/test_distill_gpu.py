@@ -25,6 +25,9 @@ CASES = [  # N, V, K, dtype, teacher, ids, temperature, softcap, layout
     (6, 501, 7, 'bf16', 'fp32', torch.int64, 1.0, 0.0, 'view'),
     (4, 300, 256, 'fp32', 'fp32', torch.int32, 1.0, 2.0, 'view'),
     (600, 777, 3, 'bf16', 'fp32', torch.int32, 1.0, 0.0, 'plain'),
+    (1500, 777, 3, 'bf16', 'fp32', torch.int32, 1.0, 0.0, 'plain'),  # more rows than CTAs of four warps: one warp a row
+    (1300, 130, 70, 'fp32', 'bf16', torch.int64, 1.0, 15.0, 'view'),
+    (1201, 5, 2, 'fp16', 'fp16', torch.int32, 2.0, 3.0, 'plain'),
 ]
 
 
@@ -99,7 +102,7 @@ def test_loss_and_gradient(case):
         assert dev[0].isfinite().all() or case[0] > 4  # the view was only read
 
 
-@pytest.mark.parametrize('N,V,K', [(2, 200003, 180), (400, 3001, 90)])
+@pytest.mark.parametrize('N,V,K', [(2, 200003, 180), (400, 3001, 90), (1400, 1201, 200)])
 def test_entries_that_repeat_or_meet_in_the_table(N, V, K):
     """More than 32 entries: ids that all fall on one place of the table of ids, each named twice and far apart; one id
     that every entry names; ids that follow one another. Twice, with equal bits."""
