@@ -338,7 +338,8 @@ int noise_qk_norm_rope(const NoiseQkNorm* args, int backward, void* workspace, s
  * sequence b at positions >= lengths[b] are padding: their keys and values are never used, whatever they
  * hold, and their query rows give zeros (lse -inf).
  * out [B, Tq, H, D] contiguous, 16-byte aligned; lse [B, H, Tq] fp32, the natural logarithm of each row's
- * sum of exp(scale q.k) over its visible keys. */
+ * sum of exp(scale q.k) over its visible keys. scale lies in [2^-100, 2^100]. Keys and values of tokens that are not
+ * padding have to be finite: a hidden one still meets a probability of 0 in its tile. */
 typedef struct NoiseWindow {
   int dtype, B, Tq, Tk, H, Hk, D, offset, window, sinks;
   float scale;

@@ -50,12 +50,11 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// Eight consecutive elements, 16-byte aligned: one 16-byte access of a 16-bit type, two of fp32.
+// Eight consecutive elements of a 16-bit type, 16-byte aligned.
 template <typename E>
 struct Vec8 {
   uint4 w;
   __device__ __forceinline__ void load(const E* p) { w = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void store(E* p) const { *reinterpret_cast<uint4*>(p) = w; }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -64,27 +63,6 @@ struct Vec8 {
       v[2 * i] = f.x, v[2 * i + 1] = f.y;
     }
   }
-  __device__ __forceinline__ void set(const float (&v)[8]) {
-    w = make_uint4(pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3]), pack2<E>(v[4], v[5]), pack2<E>(v[6], v[7]));
-  }
-  __device__ __forceinline__ void zero() { w = make_uint4(0u, 0u, 0u, 0u); }
-};
-template <>
-struct Vec8<float> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  }
-  __device__ __forceinline__ void store(float* p) const {
-    *reinterpret_cast<float4*>(p) = a, *reinterpret_cast<float4*>(p + 4) = b;
-  }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  }
-  __device__ __forceinline__ void set(const float (&v)[8]) {
-    a = make_float4(v[0], v[1], v[2], v[3]), b = make_float4(v[4], v[5], v[6], v[7]);
-  }
-  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
 };
 
 // n / d for n < 2^31 by a multiplication: with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, the quotient is
@@ -107,7 +85,6 @@ struct Vec4 {
   __device__ __forceinline__ void store(E* p) const { __stcs(reinterpret_cast<uint2*>(p), w); }
   __device__ __forceinline__ void get(float2 (&v)[2]) const { v[0] = unpack2<E>(w.x), v[1] = unpack2<E>(w.y); }
   __device__ __forceinline__ void set(const float2 (&v)[2]) { w = make_uint2(pack2<E>(v[0].x, v[0].y), pack2<E>(v[1].x, v[1].y)); }
-  __device__ __forceinline__ void zero() { w = make_uint2(0u, 0u); }
 };
 template <>
 struct Vec4<float> {
@@ -116,7 +93,6 @@ struct Vec4<float> {
   __device__ __forceinline__ void store(float* p) const { __stcs(reinterpret_cast<float4*>(p), a); }
   __device__ __forceinline__ void get(float2 (&v)[2]) const { v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w); }
   __device__ __forceinline__ void set(const float2 (&v)[2]) { a = make_float4(v[0].x, v[0].y, v[1].x, v[1].y); }
-  __device__ __forceinline__ void zero() { a = make_float4(0.f, 0.f, 0.f, 0.f); }
 };
 
 // 16 bytes of global memory into shared memory without a register; `have` false fills zeros and reads nothing.
