@@ -74,7 +74,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) { return __uint_as_float(ld_cluster_u32(addr)); }
 
-template <typename E, int DP>
+template <typename E, int DP, int kMost>  // at most kMost CTAs a cluster
 __global__ void __launch_bounds__(WinTok<DP>::kThreads) window_token_kernel(const __grid_constant__ TokenParams p) {
   using L = WinTok<DP>;
   constexpr int KC = L::KC;
@@ -236,13 +236,13 @@ __global__ void __launch_bounds__(WinTok<DP>::kThreads) window_token_kernel(cons
   for (int e = rank * L::kThreads + tid; e < heads * (DP / 2); e += parts * L::kThreads) {
     const int r = e / (DP / 2), d = (e % (DP / 2)) * 2;
     const float* row = cta + r * L::kRowFloats;
-    float top = -INFINITY, mm[8], ll[8], x[8], y[8];
+    float top = -INFINITY, mm[kMost], ll[kMost], x[kMost], y[kMost];
     if (parts == 1) {
       mm[0] = row[DP], ll[0] = row[DP + 1], x[0] = row[d], y[0] = row[d + 1];
       top = mm[0];
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < kMost; ++k) {
         if (k >= parts) break;
         const uint32_t at = cluster_addr(row, (uint32_t)k);
         mm[k] = ld_cluster_f32(at + DP * 4), ll[k] = ld_cluster_f32(at + DP * 4 + 4);
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(WinTok<DP>::kThreads) window_token_kernel(cons
     const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f, ax = 0.f, ay = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < kMost; ++k) {
       if (k >= parts) break;
       const float f = exp2f(mm[k] - base);
       sum = fmaf(ll[k], f, sum), ax = fmaf(x[k], f, ax), ay = fmaf(y[k], f, ay);
@@ -270,12 +270,28 @@ __global__ void __launch_bounds__(WinTok<DP>::kThreads) window_token_kernel(cons
 
 int check_window(const NoiseWindow* a, bool token);
 
-constexpr int kTokMaxCluster = 8;
+template <typename E, int DP, int kMost>
+static int launch_window_token(const TokenParams& p, int B, int Hk, int parts, cudaStream_t s) {
+  using L = WinTok<DP>;
+  static KernelOptIn opt_in;
+  if (!opt_in(window_token_kernel<E, DP, kMost>, L::kSmem, kMost > 8)) return kStatusLaunchFailed;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)parts, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)parts, (unsigned)(Hk * p.tiles), (unsigned)B), cfg.blockDim = dim3(L::kThreads);
+  cfg.dynamicSmemBytes = L::kSmem, cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = 1;
+  LaunchScope scope(kKindAttention, s);
+  if (cudaLaunchKernelEx(&cfg, window_token_kernel<E, DP, kMost>, p) != cudaSuccess) {
+    cudaGetLastError();
+    return kStatusLaunchFailed;
+  }
+  return kStatusOk;
+}
 
 template <typename E, int DP>
 static int launch_window_token(const NoiseWindow* a, cudaStream_t s) {
   using L = WinTok<DP>;
-  static KernelOptIn opt_in;
   TokenParams p{};
   p.q = a->q, p.k = a->k, p.v = a->v;
   p.q_b = a->q_stride[0], p.q_h = a->q_stride[2];
@@ -285,26 +301,20 @@ static int launch_window_token(const NoiseWindow* a, cudaStream_t s) {
   p.H = a->H, p.group = a->H / a->Hk, p.tiles = (p.group + 15) / 16, p.Tk = a->Tk, p.D = a->D;
   p.window = a->window < a->Tk ? a->window : a->Tk, p.sinks = a->sinks < a->Tk ? a->sinks : a->Tk;
   p.scale = a->scale;
-  // CTAs per (sequence, key head): until the GPU has two CTAs an SM, or until every warp holds one chunk
+  // CTAs per (sequence, key head): until the GPU has two CTAs an SM, or until every warp holds one chunk; 16 only where
+  // they find an SM each and every warp still has eight chunks. 8 against 16 CTAs: one sequence of 65,536 tokens, 8 key
+  // heads of 128: 96 against 76 us; of 16,384, 2 key heads of 64: 20 against 16; but of 4,096, 8 of 128: 14 against 16,
+  // and two of 8,192: 27 against 37.
   const int64_t pairs = (int64_t)a->B * a->Hk * p.tiles;
   const int64_t keys = (int64_t)p.window + 1 + p.sinks < a->Tk ? (int64_t)p.window + 1 + p.sinks : a->Tk;
   int parts = 1;
-  while (parts < kTokMaxCluster && pairs * parts < 2 * (int64_t)device_sm_count() && keys > (int64_t)parts * L::kWarps * L::KC)
+  while (parts < 8 && pairs * parts < 2 * (int64_t)device_sm_count() && keys > (int64_t)parts * L::kWarps * L::KC)
     parts *= 2;
+  if (parts == 8 && pairs * 16 <= device_sm_count() && keys >= (int64_t)16 * L::kWarps * L::KC * 8)
+    parts = 16;
   if ((int64_t)a->Hk * p.tiles > 65535) return kStatusUnsupported;
-  if (!opt_in(window_token_kernel<E, DP>, L::kSmem)) return kStatusLaunchFailed;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)parts, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)parts, (unsigned)(a->Hk * p.tiles), (unsigned)a->B), cfg.blockDim = dim3(L::kThreads);
-  cfg.dynamicSmemBytes = L::kSmem, cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = 1;
-  LaunchScope scope(kKindAttention, s);
-  if (cudaLaunchKernelEx(&cfg, window_token_kernel<E, DP>, p) != cudaSuccess) {
-    cudaGetLastError();
-    return kStatusLaunchFailed;
-  }
-  return kStatusOk;
+  return parts > 8 ? launch_window_token<E, DP, 16>(p, a->B, a->Hk, parts, s)
+                   : launch_window_token<E, DP, 8>(p, a->B, a->Hk, parts, s);
 }
 
 }  // namespace noise

@@ -262,6 +262,8 @@ TOKENS = [  # B, Tk, H, Hk, D, window, sinks, dtype, lengths
     (1, 5000, 3, 1, 128, 4000, 64, 'fp16', (4990,)),
     (70, 130, 16, 8, 40, 128, 1, 'bf16', tuple(range(61, 131))),
     (2, 333, 6, 3, 8, 0, 5, 'bf16', (333, 4)),
+    (1, 17001, 4, 2, 64, 17001, 0, 'bf16', (17001,)),     # clusters of 16 CTAs
+    (2, 9001, 20, 1, 96, 8990, 3, 'fp16', (9001, 5)),
 ]
 
 
