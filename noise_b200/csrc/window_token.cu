@@ -280,7 +280,7 @@ static int launch_window_token(const TokenParams& p, int B, int Hk, int parts, c
   attr.val.clusterDim.x = (unsigned)parts, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)parts, (unsigned)(Hk * p.tiles), (unsigned)B), cfg.blockDim = dim3(L::kThreads);
-  cfg.dynamicSmemBytes = L::kSmem, cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = 1;
+  cfg.dynamicSmemBytes = L::kSmem, cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = parts > 1;
   LaunchScope scope(kKindAttention, s);
   if (cudaLaunchKernelEx(&cfg, window_token_kernel<E, DP, kMost>, p) != cudaSuccess) {
     cudaGetLastError();
