@@ -301,14 +301,16 @@ static int launch_window_token(const NoiseWindow* a, cudaStream_t s) {
   p.H = a->H, p.group = a->H / a->Hk, p.tiles = (p.group + 15) / 16, p.Tk = a->Tk, p.D = a->D;
   p.window = a->window < a->Tk ? a->window : a->Tk, p.sinks = a->sinks < a->Tk ? a->sinks : a->Tk;
   p.scale = a->scale;
-  // CTAs per (sequence, key head): until the GPU has two CTAs an SM, or until every warp holds one chunk; 16 only where
-  // they find an SM each and every warp still has eight chunks. 8 against 16 CTAs: one sequence of 65,536 tokens, 8 key
-  // heads of 128: 96 against 76 us; of 16,384, 2 key heads of 64: 20 against 16; but of 4,096, 8 of 128: 14 against 16,
-  // and two of 8,192: 27 against 37.
+  // CTAs per (sequence, key head), a power of two: as many as the two an SM holds take in at once (twice that from one
+  // CTA to two), as long as every warp gets a chunk; 16 only where they find an SM each and every warp still has eight
+  // chunks. Twice the CTAs against these: 8 sequences of 8,192 tokens, 8 key heads of 128, 72 against 65 us; 16 of 1,024 visible
+  // ones, 8 of 64, 20 against 16; but 32 of 4,096, 8 of 128, 108 against 116 with one. 8 against 16: one of 65,536, 8 of 128,
+  // 96 against 76; one of 16,384, 2 of 64, 20 against 16; but one of 4,096, 8 of 128, 14 against 16, two of 8,192 27 against 37.
   const int64_t pairs = (int64_t)a->B * a->Hk * p.tiles;
   const int64_t keys = (int64_t)p.window + 1 + p.sinks < a->Tk ? (int64_t)p.window + 1 + p.sinks : a->Tk;
   int parts = 1;
-  while (parts < 8 && pairs * parts < 2 * (int64_t)device_sm_count() && keys > (int64_t)parts * L::kWarps * L::KC)
+  while (parts < 8 && pairs * parts <= (parts == 1 ? 2 : 1) * (int64_t)device_sm_count() &&
+         keys > (int64_t)parts * L::kWarps * L::KC)
     parts *= 2;
   if (parts == 8 && pairs * 16 <= device_sm_count() && keys >= (int64_t)16 * L::kWarps * L::KC * 8)
     parts = 16;
