@@ -12,7 +12,7 @@
 // The products run on mma.sync m16n8k16 with fp32 accumulators: a tile of at most 16 query rows leaves a
 // 128-row tensor-memory product mostly empty, and the bytes of the cache bound this form, not its products.
 // Keys behind the sequence's end are not loaded (their places read as zeros), so a cache may hold anything there.
-// Measured: 64 sequences over 8 K tokens of cache or fewer, 32 heads on 8 of 128: 183 us a call, 5.6 TB/s; one sequence,
+// Measured: 64 sequences over 8 K tokens of cache or fewer, 32 heads on 8 of 128: 173 us a call, 5.9 TB/s; one sequence,
 // 8 heads of 64, 1,024 visible keys: 11.5 us a call, which is the host's time for it.
 #include <type_traits>
 
