@@ -420,6 +420,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
       }
     };
     if (empty) {
+      cp_async_wait<0>();  // the gradient alone has not taken its first copies: they land before the CTA leaves
       float2 v[N / 2];
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) v[i] = both(0.f);
