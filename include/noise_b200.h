@@ -307,7 +307,9 @@ int noise_fitness_static(const float* losses, int members, int pairs, int mode, 
  * or t when positions is null. A position outside the table gives NaN rows. wq, wk: optional [D] fp32
  * weights of the norms. order NOISE_ROTATE_NORM: norm(R x); NOISE_NORM_ROTATE: R norm(x), with
  * R (x1, x2) = (x1 cos + x2 sin, x2 cos - x1 sin) on the halves and norm(u) = w u / sqrt(mean u^2 + eps).
- * Forward (backward = 0): q_out, k_out receive the result; they may be q and k themselves.
+ * Forward (backward = 0): q_out, k_out receive the result; they may be q and k themselves. An output that meets
+ * anything else that the call reads, the other output or its own rows is a bad argument: noise_qk_norm_overlap says so
+ * (1) without a launch.
  * Backward: dq, dk are the results' gradients, q_out and k_out receive those of q and k, dwq and dwk (given
  * exactly when wq and wk are) the weights'; a call with weights needs
  * noise_qk_norm_workspace_bytes(D) of workspace. Its sums over rows run in a fixed order. */
@@ -327,6 +329,7 @@ typedef struct NoiseQkNorm {
   float *dwq, *dwk;
 } NoiseQkNorm;
 int64_t noise_qk_norm_workspace_bytes(int D);
+int noise_qk_norm_overlap(const NoiseQkNorm* args, int backward);
 int noise_qk_norm_rope(const NoiseQkNorm* args, int backward, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Causal attention with a sliding window and `sinks` first tokens that stay visible, for any length,

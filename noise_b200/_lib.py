@@ -78,6 +78,7 @@ SIGNATURES: dict[str, tuple] = {
     'noise_fitness_static_max_members': (c_int, []),
     'noise_fitness_static': (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     'noise_qk_norm_workspace_bytes': (c_int64, [c_int]),
+    'noise_qk_norm_overlap': (c_int, [c_char_p, c_int]),
     'noise_qk_norm_rope': (c_int, [c_char_p, c_int, c_void_p, c_size_t, c_void_p]),
     'noise_window_attention': (c_int, [c_char_p, c_void_p, c_void_p]),
     'noise_window_backward_workspace_bytes': (c_int64, [c_char_p]),

@@ -164,8 +164,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, *, positi
     order 'rotate_norm' (utils/model.py:86-88): norm(R x); 'norm_rotate': R norm(x). rope is a table like
     Weights.rope: fp32 [positions, D], cos | sin; positions int32 [T] or [B, T] picks its rows (default: token
     t row t), and a position outside the table gives NaN rows. q_weight, k_weight: fp32 [D] weights of the
-    norms. out: (q_out, k_out) to write to, of any addressable layout (a cache's rows, or q and k themselves).
-    Returns (q_out, k_out)."""
+    norms. out: (q_out, k_out) to write to, of any addressable layout (a cache's rows, or q and k themselves); one that
+    overlaps anything else the call reads, the other or itself is refused. Returns (q_out, k_out)."""
     head, table, stride, qs, ks, out_steps, *_ = _qk_plan(q, k, rope, positions, q_weight, k_weight, order, eps)
     if out is None:
         q_out, k_out = _like(q), _like(k)
@@ -181,6 +181,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, *, positi
     a = _lib.QK_NORM.pack(*head, rope.data_ptr(), table, _pointer(positions), stride, _pointer(q_weight),
                           _pointer(k_weight), q.data_ptr(), k.data_ptr(), 0, 0, q_out.data_ptr(), k_out.data_ptr(), *qs, *ks,
                           *_NO_STEPS, *out_steps, 0, 0)
+    if out is not None and _lib.load().noise_qk_norm_overlap(a, 0):
+        raise ValueError('qk_norm_rope: out overlaps an input other than in place, or itself')
     launch('noise_qk_norm_rope', device, a, 0, None, 0)
     return q_out, k_out
 

@@ -22,6 +22,9 @@
 // latency at 32 warps an SM. Eight values of either half a lane save instructions and cost registers: 97 against 60 us for
 // the gradient; copies through a ring in shared memory, 68 against 58; arithmetic without pairs, 24 instructions more,
 // the same time.
+#include <algorithm>
+#include <utility>
+
 #include "operators.cuh"
 #include "profile.cuh"
 #include "ptx.cuh"
@@ -277,9 +280,109 @@ static bool qk_tensor_ok(const void* ptr, const int64_t* stride, int elem) {
   return true;
 }
 
+// Rows of `bytes` bytes at p + stride . i, 0 <= i < n.
+struct QkRows {
+  int64_t p, n[3], stride[3], bytes;
+  QkRows(const void* ptr, int B, int T, int heads, const int64_t* st, int D, int elem)
+      : p((int64_t)reinterpret_cast<uintptr_t>(ptr)), n{B, T, heads}, stride{st[0] * elem, st[1] * elem, st[2] * elem},
+        bytes((int64_t)D * elem) {}
+  bool same(const QkRows& o) const {  // the same rows in the same places
+    bool all = p == o.p;
+    for (int i = 0; i < 3; ++i) all = all && n[i] == o.n[i] && (n[i] == 1 || stride[i] == o.stride[i]);
+    return all;
+  }
+  bool within(int64_t begin, int64_t end) const {  // its extent reaches into [begin, end)
+    int64_t lo = p, hi = p + bytes;
+    for (int i = 0; i < 3; ++i) (stride[i] < 0 ? lo : hi) += (n[i] - 1) * stride[i];
+    return lo < end && begin < hi;
+  }
+};
+
+// Whether two rows meet: integers x_k in [lo_k, hi_k] with |d + sum_k step_k x_k| < bytes, and, of one set of rows against
+// itself, not all 0. The widest step first, each within what the narrower ones can still make up: two or three values a
+// step where rows are nested as in any view of a tensor. A search that gets long is taken for an overlap.
+struct QkMeet {
+  struct Step {
+    int64_t step, lo, hi;
+  } s[6];
+  int n = 0, budget = 1 << 14;
+  int64_t bytes;
+  bool self;
+
+  void add(int64_t step, int64_t lo, int64_t hi) {
+    if (step < 0) step = -step, std::swap(lo, hi), lo = -lo, hi = -hi;
+    if (!step && !self) return;  // the same rows again
+    for (int i = 0; i < n && !self; ++i)
+      if (s[i].step == step) {
+        s[i].lo += lo, s[i].hi += hi;
+        return;
+      }
+    s[n++] = {step, lo, hi};
+  }
+  bool search(int k, int64_t d, bool zero) {
+    if (--budget < 0) return true;
+    if (k == n) return d > -bytes && d < bytes && !(self && zero);
+    int64_t lo = d - bytes + 1, hi = d + bytes - 1;  // what this step has to bring to 0
+    for (int i = k + 1; i < n; ++i) lo += s[i].step * s[i].lo, hi += s[i].step * s[i].hi;
+    int64_t first = s[k].lo, last = s[k].hi;
+    if (s[k].step) {  // step x in [-hi, -lo], rounded inwards
+      auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+      first = std::max(first, -floor_div(hi, s[k].step)), last = std::min(last, floor_div(-lo, s[k].step));
+    }
+    for (int64_t x = first; x <= last; ++x)
+      if (search(k + 1, d + s[k].step * x, zero && x == 0)) return true;
+    return false;
+  }
+  static bool run(const QkRows& a, const QkRows& b, bool self) {
+    QkMeet m;
+    m.bytes = a.bytes, m.self = self;
+    for (int i = 0; i < 3; ++i) {
+      if (!a.n[i] || !b.n[i]) return false;
+      if (self) {
+        if (a.n[i] > 1) m.add(a.stride[i], -(a.n[i] - 1), a.n[i] - 1);
+        continue;
+      }
+      m.add(a.stride[i], 0, a.n[i] - 1);
+      m.add(-b.stride[i], 0, b.n[i] - 1);
+    }
+    std::sort(m.s, m.s + m.n, [](const Step& x, const Step& y) { return x.step > y.step; });
+    return m.search(0, a.p - b.p, true);
+  }
+};
+
+static bool qk_overlap(const NoiseQkNorm* a, bool backward) {
+  if (a->B < 1 || a->T < 1 || a->H < 1 || a->Hk < 1) return false;
+  const int elem = a->dtype == NOISE_FP32 ? 4 : 2;
+  auto rows = [&](const void* p, int heads, const int64_t* st) { return QkRows(p, a->B, a->T, heads, st, a->D, elem); };
+  const QkRows out[2] = {rows(a->q_out, a->H, a->q_out_stride), rows(a->k_out, a->Hk, a->k_out_stride)};
+  const QkRows in[4] = {rows(a->q, a->H, a->q_stride), rows(a->k, a->Hk, a->k_stride), rows(a->dq, a->H, a->dq_stride),
+                        rows(a->dk, a->Hk, a->dk_stride)};
+  auto apart = [](const QkRows& x, const QkRows& y) {
+    int64_t lo = y.p, hi = y.p + y.bytes;
+    for (int i = 0; i < 3; ++i) (y.stride[i] < 0 ? lo : hi) += (y.n[i] - 1) * y.stride[i];
+    return !x.within(lo, hi) || !QkMeet::run(x, y, false);
+  };
+  if (!apart(out[0], out[1])) return true;
+  for (int o = 0; o < 2; ++o) {
+    if (QkMeet::run(out[o], out[o], true)) return true;
+    for (int i = 0; i < (backward ? 4 : 2); ++i)  // a thread reads its rows before it writes them: in place is fine
+      if (!((i & 1) == o && out[o].same(in[i])) && !apart(out[o], in[i])) return true;
+    auto reads = [&](const void* p, int64_t bytes) {
+      const int64_t at = (int64_t)reinterpret_cast<uintptr_t>(p);
+      return p && out[o].within(at, at + bytes);
+    };
+    if (reads(a->rope, a->table * a->D * 4) || reads(a->wq, a->D * 4) || reads(a->wk, a->D * 4) ||
+        reads(a->positions, ((a->B - 1) * a->positions_stride + a->T) * 4))
+      return true;
+  }
+  return false;
+}
+
 }  // namespace noise
 
 using namespace noise;
+
+extern "C" int noise_qk_norm_overlap(const NoiseQkNorm* a, int backward) { return a && qk_overlap(a, backward != 0); }
 
 extern "C" int64_t noise_qk_norm_workspace_bytes(int D) {
   return D < 16 || D > 256 ? -1 : (int64_t)kQkMaxBlocks * D * 4;
@@ -308,6 +411,7 @@ extern "C" int noise_qk_norm_rope(const NoiseQkNorm* a, int backward, void* work
     return kStatusBadArgument;
   if (weights && (!workspace || workspace_bytes < (size_t)noise_qk_norm_workspace_bytes(a->D)))
     return kStatusWorkspaceTooSmall;
+  if (qk_overlap(a, backward != 0)) return kStatusBadArgument;
   QkParams p{};
   p.side[0].x = a->q, p.side[0].dy = a->dq, p.side[0].y = a->q_out, p.side[0].w = a->wq, p.side[0].heads = a->H;
   p.side[1].x = a->k, p.side[1].dy = a->dk, p.side[1].y = a->k_out, p.side[1].w = a->wk, p.side[1].heads = a->Hk;
