@@ -391,6 +391,7 @@ extern "C" int64_t noise_qk_norm_workspace_bytes(int D) {
 extern "C" int noise_qk_norm_rope(const NoiseQkNorm* a, int backward, void* workspace, size_t workspace_bytes,
                                   void* stream) {
   if (!a || !a->rope || a->B < 0 || a->T < 0 || a->H < 1 || a->Hk < 1 || a->table < 1) return kStatusBadArgument;
+  if (a->order != NOISE_ROTATE_NORM && a->order != NOISE_NORM_ROTATE) return kStatusBadArgument;
   if (a->D < 16 || a->D > 256 || a->D % 16) return kStatusUnsupported;
   if (a->dtype != NOISE_FP32 && a->dtype != NOISE_BF16 && a->dtype != NOISE_FP16) return kStatusUnsupported;
   if (a->B == 0 || a->T == 0) {  // no rows: the weights' gradients are zero
