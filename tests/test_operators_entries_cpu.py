@@ -8,4 +8,4 @@ from test_operators_cpu import qk
 def test_qk_norm_entry_refuses_an_unknown_order(order):
     """Such an order was taken for norm, then rotate."""
     from noise_b200 import _lib
-    assert _lib.load().noise_qk_norm_rope(qk(_lib.QK_NORM, order=order, q=1 << 22, k=1 << 23, ko=1 << 24), 0, None, 0, None) == 1
+    assert _lib.load().noise_qk_norm_rope(qk(_lib.QK_NORM, order=order, q=1 << 22, k=1 << 23, ko=1 << 24, rope=1 << 25), 0, None, 0, None) == 1
