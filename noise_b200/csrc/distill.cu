@@ -105,9 +105,10 @@ __device__ __forceinline__ uint4 slot_pack(const float2 (&v)[DsSlot<E>::kN / 2])
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 ex2_pair(float2 x) { return make_float2(ex2_approx(x.x), ex2_approx(x.y)); }
 
-// tanh to about 2 ulp. Up to |x| = 1 from a polynomial x + x^3 Q(x^2): Q is a least-squares fit of degree 6 at Chebyshev
-// nodes, off by 6e-9 of tanh. Beyond, where 1 - e no longer cancels, from e = exp(-2 |x|): (1 - e) / (1 + e). Logits
-// within the soft cap, nearly all of a trained model's, so take no special function for their tanh.
+// tanh to about 2 ulp and its slope 1 - tanh^2 to about (4 |x| + 8) half ulp. Up to |x| = 1 from a polynomial x + x^3 Q(x^2): Q is a least-squares fit of degree 6 at Chebyshev
+// nodes, off by 6e-9 of tanh. Beyond, where 1 - e no longer cancels, from e = exp(-2 |x|): (1 - e) / (1 + e), and the slope
+// as 4 e / (1 + e)^2, since 1 - tanh^2 would have lost all its digits at |x| = 9. Logits within the soft cap, nearly all
+// of a trained model's, so take no special function for their tanh.
 __device__ __forceinline__ float2 tanh_near(float2 x) {
   const float2 u = __fmul2_rn(x, x);
   float2 q = __ffma2_rn(both(-3.552270937e-4f), u, both(2.289985307e-3f));
@@ -118,15 +119,21 @@ __device__ __forceinline__ float2 tanh_near(float2 x) {
   q = __ffma2_rn(q, u, both(-3.333329260e-1f));
   return __ffma2_rn(__fmul2_rn(x, u), q, x);
 }
-__device__ __forceinline__ float tanh_far(float x) {
-  const float e = ex2_approx(fabsf(x) * -2.8853900817779268f);
-  return copysignf((1.f - e) * rcp_approx(1.f + e), x);
+__device__ __forceinline__ float2 slope_near(float2 th) {
+  return __ffma2_rn(make_float2(-th.x, -th.y), th, both(1.f));
 }
-__device__ __forceinline__ float2 ds_tanh(float2 x) {
-  const float2 near = tanh_near(x);
-  return make_float2(fabsf(x.x) <= 1.f ? near.x : tanh_far(x.x), fabsf(x.y) <= 1.f ? near.y : tanh_far(x.y));
+__device__ __forceinline__ float tanh_far(float x, float& slope) {
+  const float e = ex2_approx(fabsf(x) * -2.8853900817779268f), r = rcp_approx(1.f + e);
+  slope = 4.f * e * r * r;
+  return copysignf((1.f - e) * r, x);
 }
-__device__ __forceinline__ float ds_tanh(float x) { return ds_tanh(both(x)).x; }
+__device__ __forceinline__ float2 ds_tanh(float2 x, float2& slope) {
+  float2 th = tanh_near(x);
+  slope = slope_near(th);
+  if (!(fabsf(x.x) <= 1.f)) th.x = tanh_far(x.x, slope.x);
+  if (!(fabsf(x.y) <= 1.f)) th.y = tanh_far(x.y, slope.y);
+  return th;
+}
 
 // A reference m and the sum of 2^(scale (. - m)); an empty or all -inf set is (-inf, 0). The difference is taken
 // before the scale, so that values near the type's lowest do not turn into -inf.
@@ -216,20 +223,28 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
     }
   };
   start();
-  auto values = [&](float2 (&v)[N / 2]) {  // of a slot; the same numbers on either way
+  // v of a slot and, with a soft cap, its slope d v / d (z / c); the same numbers on either way
+  auto values = [&](float2 (&v)[N / 2], float2 (&slope)[N / 2]) {
     if (!kCap) return;
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) v[i] = __fmul2_rn(v[i], both(inv_cap)), top = max3(top, fabsf(v[i].x), fabsf(v[i].y));
     if (top <= 1.f) {
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) v[i] = tanh_near(v[i]);
+      for (int i = 0; i < N / 2; ++i) v[i] = tanh_near(v[i]), slope[i] = slope_near(v[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) v[i] = ds_tanh(v[i]);
+      for (int i = 0; i < N / 2; ++i) v[i] = ds_tanh(v[i], slope[i]);
     }
   };
-  auto value1 = [&](float x) { return kCap ? ds_tanh(x * inv_cap) : x; };
+  auto value1 = [&](float x, float& slope) {
+    if (!kCap) return x;
+    float2 two;
+    const float v = ds_tanh(both(x * inv_cap), two).x;
+    slope = two.x;
+    return v;
+  };
+  float unused;
 
   // Entry k: its id (-1: absent) and logit. A thread keeps its first one, k = tid, in registers from the start.
   auto entry = [&](int k, int& id) {
@@ -272,16 +287,15 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
   if constexpr (kMode != kDsGrad) {
     // one slot's sum under the reference as it stands
     auto add = [&](const uint4& w, int slot, float2& sum) {
-      float2 v[N / 2];
+      float2 v[N / 2], slope[N / 2];
       slot_values<E>(w, v);
-      values(v);
+      values(v, slope);
       if constexpr (kBound) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-          const float2 th = v[i];
-          const float2 e = ex2_pair(__ffma2_rn(th, both(scale), both(-scale)));
+          const float2 e = ex2_pair(__ffma2_rn(v[i], both(scale), both(-scale)));
           sum = __fadd2_rn(sum, e);
-          if (kHold) v[i] = __fmul2_rn(e, __ffma2_rn(make_float2(-th.x, -th.y), th, both(1.f)));
+          if (kHold) v[i] = __fmul2_rn(e, slope[i]);
         }
         if constexpr (kHold) {
 #pragma unroll
@@ -301,7 +315,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
 #pragma unroll 1
       for (int e = slot * N - phase; count; e += kDsThreads * N, --count)
 #pragma unroll 1
-        for (int i = 0; i < N; ++i) m = fmaxf(m, scale * value1(to_f32(z[e + i])));
+        for (int i = 0; i < N; ++i) m = fmaxf(m, scale * value1(to_f32(z[e + i]), unused));
       if (m > a.m) a.s = a.m == -INFINITY ? a.s : a.s * exp2f(a.m - m), a.m = m;
     };
     auto take = [&](const uint4* w, int slot, int count) {
@@ -321,7 +335,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
     };
     sweep(take);
     if (edge >= 0) {
-      const float x = value1(z_edge) * scale;
+      const float x = value1(z_edge, unused) * scale;
       if (kBound) a.s += ex2_approx(x - scale);
       else a.join(x, x == -INFINITY ? 0.f : 1.f);
     }
@@ -370,7 +384,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
       const float d = (t - top) * inv_tau, pk = exp2f((t - top) * t_scale) * inv_mass;
       // lse - s in base 2, from the difference of the reference and s
       if (id >= 0 && pk != 0.f)
-        l += pk * ((d - log_mass) + 0.6931471805599453f * (log_sum - fmaf(value1(x), scale, -a.m)));
+        l += pk * ((d - log_mass) + 0.6931471805599453f * (log_sum - fmaf(value1(x, unused), scale, -a.m)));
     };
     if (tid < p.K) term(id0, t0, z_id);
     for (int k = tid + kDsThreads; k < p.K; k += kDsThreads) {
@@ -404,10 +418,12 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
       ref = (float)lse2, low = (float)(lse2 - (double)ref), factor = 1.f;
       if (!isfinite(ref)) low = 0.f;
     }
-    // gradient at a column from v, with the entries' mass pj there
-    auto slope = [&](float v, float pj) {
+    // gradient at a column from its logit, with the entries' mass pj there
+    auto column = [&](float x, float pj) {
+      float slope;
+      const float v = value1(x, slope);
       const float d = up * fmaf(ex2_approx(fmaf(v, scale, -ref) - low), factor, -pj);
-      return kCap ? d * fmaf(-v, v, 1.0f) : d;
+      return kCap ? d * slope : d;
     };
     uint4* g16 = reinterpret_cast<uint4*>(g - phase);
     auto write = [&](int slot, const float2 (&v)[N / 2]) {
@@ -440,15 +456,15 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
           v[2 * i] = __fmul2_rn(make_float2(x.x, x.y), gain), v[2 * i + 1] = __fmul2_rn(make_float2(x.z, x.w), gain);
         }
       } else {
+        float2 slope[N / 2];
         slot_values<E>(w, v);
-        values(v);
+        values(v, slope);
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-          const float2 x = v[i];
-          float2 y = __ffma2_rn(x, both(scale), both(-ref));
+          float2 y = __ffma2_rn(v[i], both(scale), both(-ref));
           if (kMode == kDsGrad) y = __fadd2_rn(y, both(-low));
           v[i] = __fmul2_rn(ex2_pair(y), gain);
-          if (kCap) v[i] = __fmul2_rn(v[i], __ffma2_rn(make_float2(-x.x, -x.y), x, both(1.f)));
+          if (kCap) v[i] = __fmul2_rn(v[i], slope[i]);
         }
       }
       write(slot, v);
@@ -464,7 +480,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
       for (int slot = first + tid; slot < last; slot += kDsThreads)
         spread(kBound ? make_uint4(0u, 0u, 0u, 0u) : hold[slot - begin], slot);
     }
-    if (edge >= 0) g[edge] = from_f32<E>(slope(value1(z_edge), 0.f));
+    if (edge >= 0) g[edge] = from_f32<E>(column(z_edge, 0.f));
     __syncthreads();  // the dense stores of this CTA come before its entries' stores
     finish();
     const int e0 = begin * N - phase, e1 = min(p.V, end * N - phase);
@@ -475,7 +491,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
       if (again)
         for (int i = k + 1; i < p.K; ++i)
           if (s_id[i] == id) pj += exp2f((entry(i, other) - top) * t_scale) * inv_mass;
-      g[id] = from_f32<E>(slope(value1(k == tid ? z_id : to_f32(z[id])), pj));
+      g[id] = from_f32<E>(column(k == tid ? z_id : to_f32(z[id]), pj));
     };
     if (p.K <= 32) {  // equal ids by a vote of one warp
       if (warp == 0) {

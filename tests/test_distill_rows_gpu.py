@@ -1,6 +1,6 @@
-"""The distillation calls on rows that differ from their neighbours: rows without an entry between rows with entries.
+"""The distillation calls on rows without an entry between rows with entries, and on logits far beyond the soft cap.
 
-Tolerances as in test_distill_gpu.py."""
+Tolerances as in test_distill_gpu.py where nothing else is said."""
 import pytest
 import torch
 
@@ -32,3 +32,31 @@ def test_gradient_alone_of_rows_without_entries_between_others(N, V, K, cap, dty
     some = torch.arange(0, N, (N // 200) | 1)
     want, q, p, slope, E = expected(z[some], ids[some], t[some], 1.0, cap)
     check_grad(got[some.cuda()], up[some], q, p, slope, E, 1.0, dtype)
+
+
+@pytest.mark.parametrize('cap,tau', [(15.0, 1.0), (2.0, 1.0), (30.0, 0.5)])  # c / tau up to 40, and beyond
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_gradient_far_beyond_the_soft_cap(cap, tau, dtype):
+    """The slope of logits of 3 to 10 soft caps is 1e-2 to 1e-8, and as exact as any: with u = 2^-24, z / c is off by 2 u of
+    itself and the exponent 2 |z| / c by 2 u more, so the slope 4 e / (1 + e)^2 by 8 |z| / c u and the roundings of e, of
+    1 / (1 + e) twice and of the products, 20 u. What the exponentials flush to zero is below 2^-126."""
+    from noise_b200.distill import distill_backward, distill_loss, distill_loss_grad
+    g = torch.Generator().manual_seed(int(cap))
+    N, V, K = 6, 2003, 7
+    far = (3 + 7 * torch.rand(N, V, generator=g)) * (torch.randint(0, 2, (N, V), generator=g) * 2 - 1)
+    far[1] = far[1].abs()
+    far[2] = -far[2].abs()
+    far[3, ::2] *= 0.1
+    z = (far * cap).to(dtype)
+    ids, t, up = torch.randint(0, V, (N, K), generator=g), torch.randn(N, K, generator=g), torch.randn(N, generator=g)
+    _, q, p, slope, E = expected(z, ids, t, tau, cap)
+    scale = up.double().abs()[:, None] * tau
+    want = up.double()[:, None] * tau * (q - p) * slope
+    S = (8 * z.double().abs() / cap + 20) * 2.0 ** -24
+    tol = scale * slope * ((q + p) * E + (q - p).abs() * S) + torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -126 * (1 + scale)
+    dev = [x.cuda() for x in (z, ids, t)]
+    kw = dict(softcap=cap, temperature=tau)
+    _, lse = distill_loss(*dev, **kw)
+    for got in (distill_loss_grad(*dev, dloss=up.cuda(), **kw)[1], distill_backward(up.cuda(), *dev, lse, **kw)):
+        err = (got.double().cpu() - want).abs()
+        assert (err <= tol).all(), ((err / want.abs().clamp(min=1e-300))[err > tol].max(), (err > tol).sum())
