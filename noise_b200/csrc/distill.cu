@@ -10,8 +10,8 @@
 // Bound: HBM, with the issue slots and the special-function unit (16 results a cycle and SM) next: a logit takes
 // one of it, one beyond the soft cap three. The loss reads a row once. Loss and gradient
 // together read it once and write it once; the row waits between the two halves in shared memory:
-//   - with a soft cap s <= c / tau, so that is the sums' reference, no maximum is sought, and what waits is
-//     exp(s - c / tau) (1 - tanh^2), which the second half only multiplies by one factor of the row;
+//   - with a soft cap |s| <= c / tau, so the sums' reference is 0, no maximum is sought, and what waits is
+//     exp(s) (1 - tanh^2), which the second half only multiplies by one factor of the row;
 //   - without one a thread takes the maximum of its first values as its reference and looks for another only
 //     when a sum leaves fp32's safe range; what waits are the loaded words, and their exponential is taken again.
 // What it takes is bytes in flight and few instructions beside: a CTA is 128 threads, eight to an SM (one warp where
@@ -48,7 +48,8 @@ struct DsFlow {
 constexpr int kDsTable = 2 * kDsMaxK * 8 + kDsMaxK * 2;  // the table of ids, at most
 
 enum : int { kDsLoss = 0, kDsGrad = 1, kDsBoth = 2 };
-// No soft cap; one whose c / tau bounds every exponential within fp32 (2 c / tau <= 80); any other.
+// No soft cap; one whose c / tau keeps exp(s) within [e^-40, e^40], so that neither 2^30 of them nor their product with a
+// slope of 1e-19 (23 caps) leaves fp32's normal range; any other.
 enum : int { kCapNone = 0, kCapBound = 1, kCapFree = 2 };
 constexpr float kDsBoundCap = 40.f;
 
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
   }
   const float z_id = id0 >= 0 ? to_f32(z[id0]) : 0.f;
 
-  MaxSum a{kBound ? scale : -INFINITY, 0.f};
+  MaxSum a{kBound ? 0.f : -INFINITY, 0.f};
   if constexpr (kMode != kDsGrad) {
     // one slot's sum under the reference as it stands
     auto add = [&](const uint4& w, int slot, float2& sum) {
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
       if constexpr (kBound) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-          const float2 e = ex2_pair(__ffma2_rn(v[i], both(scale), both(-scale)));
+          const float2 e = ex2_pair(__fmul2_rn(v[i], both(scale)));
           sum = __fadd2_rn(sum, e);
           if (kHold) v[i] = __fmul2_rn(e, slope[i]);
         }
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
     sweep(take);
     if (edge >= 0) {
       const float x = value1(z_edge, unused) * scale;
-      if (kBound) a.s += ex2_approx(x - scale);
+      if (kBound) a.s += ex2_approx(x);
       else a.join(x, x == -INFINITY ? 0.f : 1.f);
     }
   }
