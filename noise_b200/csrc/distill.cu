@@ -52,6 +52,7 @@ enum : int { kDsLoss = 0, kDsGrad = 1, kDsBoth = 2 };
 // slope of 1e-19 (23 caps) leaves fp32's normal range; any other.
 enum : int { kCapNone = 0, kCapBound = 1, kCapFree = 2 };
 constexpr float kDsBoundCap = 40.f;
+constexpr double kDsFarLse = 1 << 29;  // lse in base 2 up to which 53 bits leave 24 behind the point
 
 struct DistillParams {
   const void* logits;
@@ -171,7 +172,9 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
   const int share = (slots + p.parts - 1) >> p.shift;
   const int begin = min(slots, rank * share), end = min(slots, begin + share);
   const float inv_tau = p.inv_tau, inv_cap = p.inv_cap;
-  // s in base 2 is scale * v, with v = z, or tanh(z / c)
+  // s in base 2 is scale * v, with v = z, or tanh(z / c). References are values of v, and v's difference from one is
+  // taken before the scale: a row whose every logit is a mask's -1e30, or the type's lowest value, then has the sums of a
+  // row of equal logits, where scale * v has lost them or is -inf.
   const float scale = (kCap ? p.cap : 1.f) * inv_tau * kLog2e;
 
   // This CTA's whole slots, and its share of the row's at most two partial ones, an element a thread: the head's by
@@ -307,7 +310,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
       } else {
         const float2 off = both(a.m == -INFINITY ? 0.f : -a.m);
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) sum = __fadd2_rn(sum, ex2_pair(__ffma2_rn(v[i], both(scale), off)));
+        for (int i = 0; i < N / 2; ++i) sum = __fadd2_rn(sum, ex2_pair(__fmul2_rn(__fadd2_rn(v[i], off), both(scale))));
       }
     };
     // a reference that the slots from `slot` on, `count` of them, do not overflow
@@ -316,8 +319,8 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
 #pragma unroll 1
       for (int e = slot * N - phase; count; e += kDsThreads * N, --count)
 #pragma unroll 1
-        for (int i = 0; i < N; ++i) m = fmaxf(m, scale * value1(to_f32(z[e + i]), unused));
-      if (m > a.m) a.s = a.m == -INFINITY ? a.s : a.s * exp2f(a.m - m), a.m = m;
+        for (int i = 0; i < N; ++i) m = fmaxf(m, value1(to_f32(z[e + i]), unused));
+      if (m > a.m) a.s = a.m == -INFINITY ? a.s : a.s * exp2f((a.m - m) * scale), a.m = m;
     };
     auto take = [&](const uint4* w, int slot, int count) {
       if (!kBound && a.m == -INFINITY) raise(slot, count);
@@ -336,9 +339,9 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
     };
     sweep(take);
     if (edge >= 0) {
-      const float x = value1(z_edge, unused) * scale;
-      if (kBound) a.s += ex2_approx(x);
-      else a.join(x, x == -INFINITY ? 0.f : 1.f);
+      const float x = value1(z_edge, unused);
+      if (kBound) a.s += ex2_approx(x * scale);
+      else a.join(x, x == -INFINITY ? 0.f : 1.f, scale);
     }
   }
 #pragma unroll
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
     if (kMode == kDsGrad) break;
     const float os = __shfl_xor_sync(0xffffffffu, a.s, o);
     if (kBound) a.s += os;
-    else a.join(__shfl_xor_sync(0xffffffffu, a.m, o), os);
+    else a.join(__shfl_xor_sync(0xffffffffu, a.m, o), os, scale);
   }
   if (lane == 0) red[0][warp] = a.m, red[1][warp] = a.s;
   __syncthreads();
@@ -362,7 +365,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
 #pragma unroll
     for (int w = 1; w < kDsWarps; ++w) {
       if (kBound) a.s += red[1][w];
-      else a.join(red[0][w], red[1][w]);
+      else a.join(red[0][w], red[1][w], scale);
     }
     if (p.parts > 1) {
       if (tid == 0) part = make_float2(a.m, a.s);
@@ -370,7 +373,7 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
       MaxSum all{-INFINITY, 0.f};
       for (int r = 0; r < p.parts; ++r) {
         const uint32_t at = cluster_addr(&part, (uint32_t)r);
-        all.join(__uint_as_float(ld_cluster_u32(at)), __uint_as_float(ld_cluster_u32(at + 4)));
+        all.join(__uint_as_float(ld_cluster_u32(at)), __uint_as_float(ld_cluster_u32(at + 4)), scale);
       }
       a = all;
       cluster_sync();  // no CTA of the cluster leaves while another reads its part
@@ -379,13 +382,13 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
 
   // the loss's terms, added up behind the dense gradient
   if (kMode != kDsGrad && rank == 0 && warp * 32 < p.K) {
-    const float log_mass = logf(mass), log_sum = log2f(a.s);
+    const float log_mass = logf(mass), log_sum = logf(a.s);
     float l = 0.f;
     auto term = [&](int id, float t, float x) {
       const float d = (t - top) * inv_tau, pk = exp2f((t - top) * t_scale) * inv_mass;
-      // lse - s in base 2, from the difference of the reference and s
+      // tau times the term, with lse - s from the difference of v and the reference: finite wherever the loss is
       if (id >= 0 && pk != 0.f)
-        l += pk * ((d - log_mass) + 0.6931471805599453f * (log_sum - fmaf(value1(x, unused), scale, -a.m)));
+        l += pk * (p.tau * ((d - log_mass) + log_sum) - (value1(x, unused) - a.m) * (kCap ? p.cap : 1.f));
     };
     if (tid < p.K) term(id0, t0, z_id);
     for (int k = tid + kDsThreads; k < p.K; k += kDsThreads) {
@@ -403,27 +406,48 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
 #pragma unroll
     for (int w = 1; w < kDsWarps; ++w)
       if (w * 32 < p.K) l += red[4][w];
-    p.loss[row] = empty ? 0.f : p.tau * p.tau * l;
+    p.loss[row] = empty ? 0.f : p.tau * l;
     // in 64 bits: the gradient's exponentials have the error of this number in common
-    if (p.lse) p.lse[row] = 0.6931471805599453094 * ((double)a.m + log2((double)a.s));
+    if (p.lse) p.lse[row] = 0.6931471805599453094 * ((double)a.m * (double)scale + log2((double)a.s));
   };
 
   if constexpr (kMode != kDsLoss) {
     E* g = reinterpret_cast<E*>(p.grad) + row * p.grad_ld;
     const bool same = (int)((reinterpret_cast<uintptr_t>(g) & 15) / sizeof(E)) == phase;
     const float up = empty ? 0.f : p.tau * (p.up ? __ldg(p.up + row) : 1.0f);
-    // softmax(s) is 2^(scale v - ref - low) * factor
+    // softmax(s) is 2^(scale (v - ref) - low) * factor
     float ref = a.m, low = 0.f, factor = 1.f / a.s;
     if constexpr (kMode == kDsGrad) {
       const double lse2 = p.lse_in[row] * 1.4426950408889634074;
-      ref = (float)lse2, low = (float)(lse2 - (double)ref), factor = 1.f;
-      if (!isfinite(ref)) low = 0.f;
+      ref = (float)(lse2 / (double)scale), low = (float)(lse2 - (double)ref * (double)scale), factor = 1.f;
+      if (!isfinite(ref)) ref = 0.f, low = (float)lse2;
+      if (isfinite(lse2) && !(fabs(lse2) < kDsFarLse) && !empty) {
+        // so far out that lse in 64 bits has not the 24 bits left that the gradient needs: the row's sum once more, by
+        // every CTA of the row for itself
+        MaxSum far{-INFINITY, 0.f};
+        for (int e = tid; e < p.V; e += kDsThreads) {
+          const float v = value1(to_f32(z[e]), unused);
+          far.join(v, v == -INFINITY ? 0.f : 1.f, scale);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+          const float os = __shfl_xor_sync(0xffffffffu, far.s, o);
+          far.join(__shfl_xor_sync(0xffffffffu, far.m, o), os, scale);
+        }
+        __syncthreads();  // red's last readers are done
+        if (lane == 0) red[0][warp] = far.m, red[1][warp] = far.s;
+        __syncthreads();
+        far = MaxSum{red[0][0], red[1][0]};
+#pragma unroll
+        for (int w = 1; w < kDsWarps; ++w) far.join(red[0][w], red[1][w], scale);
+        ref = far.m, low = 0.f, factor = 1.f / far.s;
+      }
     }
     // gradient at a column from its logit, with the entries' mass pj there
     auto column = [&](float x, float pj) {
       float slope;
       const float v = value1(x, slope);
-      const float d = up * fmaf(ex2_approx(fmaf(v, scale, -ref) - low), factor, -pj);
+      const float d = up * fmaf(ex2_approx(fmaf(v - ref, scale, -low)), factor, -pj);
       return kCap ? d * slope : d;
     };
     uint4* g16 = reinterpret_cast<uint4*>(g - phase);
@@ -462,8 +486,8 @@ __global__ void __launch_bounds__(kDsThreads, kDsSmThreads / kDsThreads) distill
         values(v, slope);
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-          float2 y = __ffma2_rn(v[i], both(scale), both(-ref));
-          if (kMode == kDsGrad) y = __fadd2_rn(y, both(-low));
+          const float2 away = __fadd2_rn(v[i], both(-ref));
+          const float2 y = kMode == kDsGrad ? __ffma2_rn(away, both(scale), both(-low)) : __fmul2_rn(away, both(scale));
           v[i] = __fmul2_rn(ex2_pair(y), gain);
           if (kCap) v[i] = __fmul2_rn(v[i], slope[i]);
         }

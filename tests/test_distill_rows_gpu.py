@@ -1,9 +1,11 @@
-"""The distillation calls on rows without an entry between rows with entries, and on logits far beyond the soft cap.
+"""The distillation calls on rows without an entry between rows with entries, on logits far beyond the soft cap, and
+on rows that a mask covers.
 
 Tolerances as in test_distill_gpu.py where nothing else is said."""
 import pytest
 import torch
 
+from oracle import operators as oo
 from test_distill_gpu import check_grad, expected
 
 pytestmark = pytest.mark.gpu
@@ -62,3 +64,44 @@ def test_gradient_far_beyond_the_soft_cap(cap, tau, dtype):
     for got in (distill_loss_grad(*dev, dloss=up.cuda(), **kw)[1], distill_backward(up.cuda(), *dev, lse, **kw)):
         err = (got.double().cpu() - want).abs()
         assert (err <= tol).all(), ((err / want.abs().clamp(min=1e-300))[err > tol].max(), (err > tol).sum())
+
+
+@pytest.mark.parametrize('mask', ['lowest', -1e30, -1e10, -60000.0])
+@pytest.mark.parametrize('N,V,dtype,tau', [(6, 2003, torch.float32, 1.0), (6, 70001, torch.bfloat16, 0.5),
+                                           (1500, 333, torch.float32, 2.0), (1500, 333, torch.float16, 1.0)])
+def test_rows_masked_as_a_whole(mask, N, V, dtype, tau):
+    """Logits that are a mask's value, or the type's lowest, in a whole row, in all but a few columns, and beside half of it:
+    the row is that of its differences, and a row whose loss has no weight gets zeros, not NaN. The differences between
+    columns that count are 0 or of normal size, so the relative error is that of normal logits:
+    E = 2^-20 + 12 * 2^-24 * 20 / temperature + (V / 1024 + 16) 2^-24."""
+    from noise_b200.distill import distill_backward, distill_loss, distill_loss_grad
+    mask = torch.finfo(dtype).min if mask == 'lowest' else max(mask, torch.finfo(dtype).min)
+    g = torch.Generator().manual_seed(V)
+    K = 5
+    z = torch.randn(N, V, generator=g).mul_(2).to(dtype)
+    z[0::6] = mask
+    z[1::6, 3:] = mask                      # its entries lie on masked columns, all but one
+    z[2::6, 1::2] = mask
+    z[3::6] = mask
+    z[4::6], z[4::6, ::2] = mask, mask / 2  # half of the row counts
+    z[5::6, 5:] = -torch.inf
+    z[5::6, :5] = mask
+    ids, t, up = torch.randint(0, V, (N, K), generator=g), torch.randn(N, K, generator=g), torch.randn(N, generator=g)
+    ids[1::6, 0] = 1
+    ids[4::6] = ids[4::6] // 2 * 2          # (an entry that does not count has a loss beyond the type)
+    ids[5::6] = ids[5::6] % 5
+    up[3::6] = 0.0
+    want, q, p, _ = oo.distill(z, ids, t, tau)
+    E = 2.0 ** -20 + 12 * 2.0 ** -24 * 20 / tau + (V / 1024 + 16) * 2.0 ** -24
+    dev = [x.cuda() for x in (z, ids, t)]
+    loss, lse = distill_loss(*dev, temperature=tau)
+    both, grad = distill_loss_grad(*dev, dloss=up.cuda(), temperature=tau)
+    for got in (loss, both):
+        got = got.double().cpu()
+        fits, beyond = want < 3.4e38, want > 3.41e38  # fp32 ends at 3.403e38
+        assert ((got - want).abs() <= 2 * tau * tau * E + 2.0 ** -20 * want.abs())[fits].all()
+        assert (got[beyond] == torch.inf).all()
+    slope = torch.ones_like(q)
+    for got in (grad, distill_backward(up.cuda(), *dev, lse, temperature=tau)):
+        check_grad(got, up, q, p, slope, E, tau, dtype)
+        assert (got[3::6] == 0).all()
