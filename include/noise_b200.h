@@ -368,6 +368,9 @@ int noise_window_attention_backward(const NoiseWindow* args, const void* dout, c
  * value are in the cache. lengths[b] = 0 gives zeros. Tq and offset are not read. out [B, H, D]
  * contiguous; lse [B, H] fp32, optional. */
 int noise_window_token(const NoiseWindow* args, void* stream);
+/* The CTAs that it gives each sequence and key head (and 16 query heads) on a device of `sms` SMs that places clusters of up
+ * to `widest` CTAs: 8 everywhere, 16 where the device says so. -1 for arguments that noise_window_token refuses. */
+int noise_window_token_ctas(const NoiseWindow* args, int sms, int widest);
 
 /* Distillation from a teacher's top logits. logits [N, V] (row stride ld) of `dtype`, ids [N, K] int32 or
  * int64 (row stride ids_ld), teacher [N, K] logits of teacher_dtype (row stride teacher_ld), K <= 1024.

@@ -85,6 +85,7 @@ SIGNATURES: dict[str, tuple] = {
     'noise_window_attention_backward': (c_int, [c_char_p, c_void_p, c_char_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                                 c_size_t, c_void_p, c_void_p]),
     'noise_window_token': (c_int, [c_char_p, c_void_p]),
+    'noise_window_token_ctas': (c_int, [c_char_p, c_int, c_int]),
     'noise_distill_max_vocab': (c_int64, [c_int, c_int]),
     'noise_distill': (c_int, [c_char_p, c_void_p]),
     'noise_launch_count': (c_int64, []),

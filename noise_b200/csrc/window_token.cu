@@ -14,6 +14,7 @@
 // Keys behind the sequence's end are not loaded (their places read as zeros), so a cache may hold anything there.
 // Measured: 64 sequences over 8 K tokens of cache or fewer, 32 heads on 8 of 128: 173 us a call, 5.9 TB/s; one sequence,
 // 8 heads of 64, 1,024 visible keys: 11.5 us a call, which is the host's time for it.
+#include <atomic>
 #include <type_traits>
 
 #include "profile.cuh"
@@ -270,6 +271,21 @@ __global__ void __launch_bounds__(WinTok<DP>::kThreads) window_token_kernel(cons
 
 int check_window(const NoiseWindow* a, bool token);
 
+// CTAs per (sequence, key head), a power of two: as many as the two an SM holds take in at once (twice that from one
+// CTA to two), as long as every warp gets a chunk; 16 only where they find an SM each and every warp still has eight
+// chunks. Twice the CTAs against these: 8 sequences of 8,192 tokens, 8 key heads of 128, 72 against 65 us; 16 of 1,024 visible
+// ones, 8 of 64, 20 against 16; but 32 of 4,096, 8 of 128, 108 against 116 with one. 8 against 16: one of 65,536, 8 of 128,
+// 96 against 76; one of 16,384, 2 of 64, 20 against 16; but one of 4,096, 8 of 128, 14 against 16, two of 8,192 27 against 37.
+static int token_ctas(const NoiseWindow* a, int sms, int widest) {
+  const int window = a->window < a->Tk ? a->window : a->Tk, sinks = a->sinks < a->Tk ? a->sinks : a->Tk;
+  const int64_t pairs = (int64_t)a->B * a->Hk * ((a->H / a->Hk + 15) / 16);
+  const int64_t keys = (int64_t)window + 1 + sinks < a->Tk ? (int64_t)window + 1 + sinks : a->Tk;
+  const int64_t chunks = a->D <= 64 ? WinTok<64>::kWarps * WinTok<64>::KC : WinTok<128>::kWarps * WinTok<128>::KC;
+  int parts = 1;
+  while (parts < 8 && pairs * parts <= (parts == 1 ? 2 : 1) * (int64_t)sms && keys > parts * chunks) parts *= 2;
+  return parts == 8 && widest >= 16 && pairs * 16 <= sms && keys >= 16 * chunks * 8 ? 16 : parts;
+}
+
 template <typename E, int DP, int kMost>
 static int launch_window_token(const TokenParams& p, int B, int Hk, int parts, cudaStream_t s) {
   using L = WinTok<DP>;
@@ -281,6 +297,18 @@ static int launch_window_token(const TokenParams& p, int B, int Hk, int parts, c
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)parts, (unsigned)(Hk * p.tiles), (unsigned)B), cfg.blockDim = dim3(L::kThreads);
   cfg.dynamicSmemBytes = L::kSmem, cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = parts > 1;
+  if constexpr (kMost > 8) {  // more CTAs than every device places: asked for once a device
+    static std::atomic<uint64_t> placed{0}, not_placed{0};
+    int dev = 0, clusters = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return kStatusLaunchFailed;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!((placed.load() | not_placed.load()) & bit)) {
+      if (cudaOccupancyMaxActiveClusters(&clusters, window_token_kernel<E, DP, kMost>, &cfg) != cudaSuccess)
+        cudaGetLastError(), clusters = 0;
+      (clusters > 0 ? placed : not_placed).fetch_or(bit);
+    }
+    if (not_placed.load() & bit) return kStatusUnsupported;
+  }
   LaunchScope scope(kKindAttention, s);
   if (cudaLaunchKernelEx(&cfg, window_token_kernel<E, DP, kMost>, p) != cudaSuccess) {
     cudaGetLastError();
@@ -301,27 +329,23 @@ static int launch_window_token(const NoiseWindow* a, cudaStream_t s) {
   p.H = a->H, p.group = a->H / a->Hk, p.tiles = (p.group + 15) / 16, p.Tk = a->Tk, p.D = a->D;
   p.window = a->window < a->Tk ? a->window : a->Tk, p.sinks = a->sinks < a->Tk ? a->sinks : a->Tk;
   p.scale = a->scale;
-  // CTAs per (sequence, key head), a power of two: as many as the two an SM holds take in at once (twice that from one
-  // CTA to two), as long as every warp gets a chunk; 16 only where they find an SM each and every warp still has eight
-  // chunks. Twice the CTAs against these: 8 sequences of 8,192 tokens, 8 key heads of 128, 72 against 65 us; 16 of 1,024 visible
-  // ones, 8 of 64, 20 against 16; but 32 of 4,096, 8 of 128, 108 against 116 with one. 8 against 16: one of 65,536, 8 of 128,
-  // 96 against 76; one of 16,384, 2 of 64, 20 against 16; but one of 4,096, 8 of 128, 14 against 16, two of 8,192 27 against 37.
-  const int64_t pairs = (int64_t)a->B * a->Hk * p.tiles;
-  const int64_t keys = (int64_t)p.window + 1 + p.sinks < a->Tk ? (int64_t)p.window + 1 + p.sinks : a->Tk;
-  int parts = 1;
-  while (parts < 8 && pairs * parts <= (parts == 1 ? 2 : 1) * (int64_t)device_sm_count() &&
-         keys > (int64_t)parts * L::kWarps * L::KC)
-    parts *= 2;
-  if (parts == 8 && pairs * 16 <= device_sm_count() && keys >= (int64_t)16 * L::kWarps * L::KC * 8)
-    parts = 16;
   if ((int64_t)a->Hk * p.tiles > 65535) return kStatusUnsupported;
-  return parts > 8 ? launch_window_token<E, DP, 16>(p, a->B, a->Hk, parts, s)
-                   : launch_window_token<E, DP, 8>(p, a->B, a->Hk, parts, s);
+  const int sms = device_sm_count(), parts = token_ctas(a, sms, 16);
+  if (parts > 8) {
+    const int rc = launch_window_token<E, DP, 16>(p, a->B, a->Hk, parts, s);
+    if (rc != kStatusUnsupported) return rc;
+  }
+  return launch_window_token<E, DP, 8>(p, a->B, a->Hk, token_ctas(a, sms, 8), s);
 }
 
 }  // namespace noise
 
 using namespace noise;
+
+extern "C" int noise_window_token_ctas(const NoiseWindow* a, int sms, int widest) {
+  const int rc = check_window(a, true);
+  return rc != kStatusOk || a->B == 0 || sms < 1 ? -1 : token_ctas(a, sms, widest);
+}
 
 extern "C" int noise_window_token(const NoiseWindow* a, void* stream) {
   const int rc = check_window(a, true);
