@@ -348,22 +348,24 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
 
 
 def window_attention_token(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor,
-                           window: int | None, sinks: int = 0, *, scale: float | None = None) -> torch.Tensor:
+                           window: int | None, sinks: int = 0, *, scale: float | None = None, with_lse: bool = False):
     """The newest token of each sequence over a cache: q [B, H, D], k and v [B, Tk, Hk, D], lengths int32 [B]. The
     query of sequence b is at position lengths[b] - 1, its own key and value included in the cache, and sees what
-    window_attention would show it; only those keys are read. lengths[b] = 0 gives zeros. Returns out [B, H, D]."""
+    window_attention would show it; only those keys are read. lengths[b] = 0 gives zeros (lse -inf). Returns out [B, H, D],
+    with with_lse (out, lse fp32 [B, H])."""
     name = 'window_attention_token'
     if lengths is None:
         raise ValueError(f'{name}: lengths are required')
     head, qs, ks, vs, _ = _window_plan(name, q, k, v, window, sinks, lengths, None, scale, True)
     device = device_index(name, q, k, v, lengths)
     out = _like(q)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if with_lse else None
     if not out.numel():
-        return out
+        return (out, lse) if with_lse else out
     if qs is None or q.data_ptr() & 15:
         q, qs = q.clone(memory_format=torch.contiguous_format), (q.shape[1] * q.shape[2], 0, q.shape[2])
     (k, ks), (v, vs) = _rows(k, ks), _rows(v, vs)
     a = _lib.WINDOW.pack(*head, lengths.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs,
-                         out.data_ptr(), 0)
+                         out.data_ptr(), _pointer(lse))
     launch('noise_window_token', device, a)
-    return out
+    return (out, lse) if with_lse else out

@@ -1,0 +1,35 @@
+"""The sliding-window attention where test_window_gpu.py does not look: the token form's lse."""
+import pytest
+import torch
+
+from oracle import operators as oo
+from test_window_gpu import DT, TOKENS, deltas, randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('case', TOKENS)
+def test_token_lse(case):
+    """|lse - want| within delta (test_window_gpu.py: the relative error of the probabilities' sum) and its own rounding."""
+    from noise_b200.attention import window_attention_token
+    B, Tk, H, Hk, D, window, sinks, dt, lengths = case
+    g = torch.Generator().manual_seed(B + Tk + D)
+    q, k, v = randn(g, B, H, D, dtype=DT[dt]), randn(g, B, Tk, Hk, D, dtype=DT[dt]), randn(g, B, Tk, Hk, D, dtype=DT[dt])
+    ln = torch.tensor(lengths, dtype=torch.int32).cuda()
+    args = (q.cuda(), k.cuda(), v.cuda(), ln, window, sinks)
+    out, lse = window_attention_token(*args, with_lse=True)
+    assert torch.equal(out, window_attention_token(*args)) and lse.shape == (B, H) and lse.dtype == torch.float32
+    d = deltas(q, k)
+    for b, n in enumerate(lengths):
+        if n == 0:
+            assert (lse[b] == -torch.inf).all()
+            continue
+        want = oo.window_attention(q[b:b + 1, None], k[b:b + 1, :n], v[b:b + 1, :n], window, sinks)[1][0, :, 0]
+        assert ((lse[b].double().cpu() - want).abs() <= d + 2.0 ** -22 * want.abs() + 2.0 ** -21).all(), b
+
+
+def test_token_lse_of_an_empty_batch():
+    from noise_b200.attention import window_attention_token
+    z = torch.zeros(0, 5, 2, 64, dtype=torch.bfloat16, device='cuda')
+    out, lse = window_attention_token(z[:, 0], z, z, torch.zeros(0, dtype=torch.int32, device='cuda'), 3, with_lse=True)
+    assert out.shape == (0, 2, 64) and lse.shape == (0, 2)
