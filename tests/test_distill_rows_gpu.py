@@ -105,3 +105,21 @@ def test_rows_masked_as_a_whole(mask, N, V, dtype, tau):
     for got in (grad, distill_backward(up.cuda(), *dev, lse, temperature=tau)):
         check_grad(got, up, q, p, slope, E, tau, dtype)
         assert (got[3::6] == 0).all()
+
+
+@pytest.mark.parametrize('N,V,dtype', [(6, 501, torch.bfloat16), (1300, 130, torch.float32), (3, 70001, torch.float16)])
+def test_inputs_are_only_read(N, V, dtype):
+    """Logits that are columns of a wider matrix: its bits stay, those around the view among them."""
+    from noise_b200.distill import distill_backward, distill_loss, distill_loss_grad
+    g = torch.Generator().manual_seed(V)
+    wide = torch.full((N + 2, V + 5), float('nan'), dtype=dtype, device='cuda')
+    z = wide[1:-1, 3:3 + V]
+    z.copy_(torch.randn(N, V, generator=g))
+    ids, t = torch.randint(0, V, (N, 7), generator=g).cuda(), torch.randn(N, 7, generator=g).cuda()
+    bits = {2: torch.int16, 4: torch.int32}[wide.element_size()]
+    before = wide.view(bits).clone(), ids.clone(), t.clone()
+    for cap in (0.0, 15.0):
+        loss, lse = distill_loss(z, ids, t, softcap=cap)
+        distill_loss_grad(z, ids, t, softcap=cap)
+        distill_backward(torch.ones_like(loss), z, ids, t, lse, softcap=cap)
+    assert torch.equal(wide.view(bits), before[0]) and torch.equal(ids, before[1]) and torch.equal(t, before[2])
