@@ -464,8 +464,10 @@ def exact_local_errors(w: Weights, cap: Capture, targets: dict, kinds=tuple(LOCA
                        inputs: dict | None = None) -> dict[str, dict[str, torch.Tensor]]:
     """The errors that local_errors estimates, without draws: {kind: {site: [B, T, width]}}, the gradients of
     sum <targets[layer], attention output> with respect to each block's raw queries and keys, values, gate logits and
-    value-embedding rows. local_errors converges to them as its draws grow and sigma shrinks, for gamma = 1 where
-    a score is spread over tokens (its credit decays by gamma a token). Every rank gets the same errors."""
+    value-embedding rows. local_errors converges to them as its draws grow and sigma shrinks at gamma = 1. DUST's
+    steps draw at gamma = 0.98, whose credit decays with the distance of the later token: of k, v, gate and ve they
+    estimate a damped error (at 128 tokens its part along the exact one is 0.7 to 0.8), of q the same. A step with these errors is
+    not forward-only. Every rank gets the same errors."""
     dev, B, T = w.device, cap.B, cap.T
     shape = (B, T, HEADS, HEAD_DIM)
     rope = w.rope(T)

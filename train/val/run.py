@@ -43,7 +43,8 @@ def main(track: str = 'val', default_scale: float = 1.0, target: float | None = 
     parser.add_argument('--eval-every', type=int, default=0, help='Untimed validation every this many updates.')
     parser.add_argument('--synthetic', action='store_true', help='Zipf(1.1) rows when the FineWeb files are absent.')
     parser.add_argument('--exact-local', action='store_true',
-                        help='Attention-internal errors from their gradients instead of draws (how much the draws cost).')
+                        help='Attention-internal errors from their gradients instead of draws, and without the draws\' decay '
+                             'of credit (gamma). A comparison run: it is no longer trained by forward passes alone.')
     args = parser.parse_args()
 
     if not torch.cuda.is_available():
