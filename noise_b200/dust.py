@@ -302,7 +302,8 @@ def distill_error(cap: Capture, ids: torch.Tensor, teacher: torch.Tensor, temper
     """The captured head against a teacher's top logits instead of the targets: ids and teacher [B, T, K] -> each
     token's distillation loss [B, T] and the head's output error [B, T, 4096], the losses' exact gradient with
     respect to the raw logits (what head_error is to the targets' loss; reassemble turns it into lm_head's
-    gradient). Tokens whose target is ignored (< 0) have error 0."""
+    gradient). Tokens whose target is ignored (< 0) have error 0; the losses are of every token, as the capture's are, and a
+    mean that the error belongs to takes those with a target."""
     k = ids.shape[-1]
     loss, error = distill_loss_grad(cap.logits, ids.reshape(-1, k), teacher.reshape(-1, k), temperature=temperature,
                                     softcap=SOFTCAP, dloss=(cap.y.reshape(-1) >= 0).float())

@@ -43,3 +43,28 @@ def test_decay_is_not_what_the_exact_errors_have():
     drawn = local_errors(w, cap, 'v', 32768, targets, 0, 1)
     for site, e in exact.items():
         assert 0.3 < measures(e, drawn[site])[1] < 0.95
+
+
+def test_distillation_error_belongs_to_the_mean_over_targets():
+    """Differences of the losses' sum over the tokens with a target give the error; the others' losses are there, their
+    error is 0. The largest error per token is about 1, a step of 0.05 on fp32 logits leaves 1e-3 (h^2 / 6 of the third
+    derivative, below 1, and 2^-20 of a loss of 20 over h)."""
+    from noise_b200.dust import distill_error
+    from test_operators_chain_gpu import _capture
+    w, cap = _capture(1, 128)
+    cap.y[0, 3] = -1
+    g = torch.Generator().manual_seed(24)
+    ids = torch.randint(0, 4096, (1, 128, 8), generator=g).cuda()
+    t = (torch.randn(1, 128, 8, generator=g) * 2).cuda()
+    loss, err = distill_error(cap, ids, t)
+    assert loss[0, 3] > 0 and (err[0, 3] == 0).all()
+    clean, h = cap.logits.clone(), 0.05
+    for token in (0, 3, 77):
+        at = int(ids[0, token, 0])
+        ends = []
+        for step in (h, -h):
+            cap.logits.copy_(clean)
+            cap.logits.view(128, 4096)[token, at] += step
+            ends.append(distill_error(cap, ids, t)[0][cap.y >= 0].double().sum().item())
+        assert abs((ends[0] - ends[1]) / (2 * h) - err[0, token, at].item()) < 2e-3, token
+    cap.logits.copy_(clean)
