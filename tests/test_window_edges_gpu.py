@@ -1,4 +1,4 @@
-"""The sliding-window attention where test_window_gpu.py does not look: the token form's lse."""
+"""The sliding-window attention where test_window_gpu.py does not look: the token form's lse and the bits of its P."""
 import pytest
 import torch
 
@@ -33,3 +33,26 @@ def test_token_lse_of_an_empty_batch():
     z = torch.zeros(0, 5, 2, 64, dtype=torch.bfloat16, device='cuda')
     out, lse = window_attention_token(z[:, 0], z, z, torch.zeros(0, dtype=torch.int32, device='cuda'), 3, with_lse=True)
     assert out.shape == (0, 2, 64) and lse.shape == (0, 2)
+
+
+@pytest.mark.parametrize('case', TOKENS)
+def test_token_probabilities_have_two_parts(case):
+    """P goes into its product as two numbers of the input type, so all of the error but the result's own rounding is fp32's
+    delta and what the second part leaves: 2^-16 of bf16 (two roundings of 2^-8), 2^-22 of fp16 with the subnormal half
+    step 2^-25 for each key. test_window_gpu.py grants one part, u sum p |v|, 256 times as much in bf16."""
+    from noise_b200.attention import window_attention_token
+    B, Tk, H, Hk, D, window, sinks, dt, lengths = case
+    g = torch.Generator().manual_seed(B + Tk + D)
+    q, k, v = randn(g, B, H, D, dtype=DT[dt]) / 8, randn(g, B, Tk, Hk, D, dtype=DT[dt]), randn(g, B, Tk, Hk, D, dtype=DT[dt])
+    ln = torch.tensor(lengths, dtype=torch.int32).cuda()
+    out = window_attention_token(q.cuda(), k.cuda(), v.cuda(), ln, window, sinks)
+    u, d = torch.finfo(DT[dt]).eps / 2, deltas(q, k)
+    for b, n in enumerate(lengths):
+        if not n:
+            continue
+        want, _, mag = oo.window_attention(q[b:b + 1, None], k[b:b + 1, :n], v[b:b + 1, :n], window, sinks)
+        tol = (u * u + d) * mag + u * want.abs()
+        if dt == 'fp16':
+            tol = tol + (n * v.double().abs().max() + 1) * 2.0 ** -25
+        err = (out[b].double().cpu() - want[0, 0]).abs()
+        assert (err <= tol[0, 0]).all(), (b, (err / tol[0, 0]).max())
