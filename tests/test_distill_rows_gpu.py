@@ -123,3 +123,24 @@ def test_inputs_are_only_read(N, V, dtype):
         distill_loss_grad(z, ids, t, softcap=cap)
         distill_backward(torch.ones_like(loss), z, ids, t, lse, softcap=cap)
     assert torch.equal(wide.view(bits), before[0]) and torch.equal(ids, before[1]) and torch.equal(t, before[2])
+
+
+@pytest.mark.parametrize('dtype,cap', [(torch.float32, 0.0), (torch.float32, 15.0), (torch.bfloat16, 0.0), (torch.float16, 50.0)])
+@pytest.mark.parametrize('K', [3, 1024])
+def test_the_longest_rows_that_one_pass_takes(dtype, cap, K):
+    """noise_distill_max_vocab logits a row: a cluster of 8 CTAs whose shared memory is full."""
+    from noise_b200 import _lib
+    from noise_b200.distill import distill_loss, distill_loss_grad
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    V = int(_lib.load().noise_distill_max_vocab(code, int(cap > 0)))
+    g = torch.Generator().manual_seed(K)
+    wide = torch.randn(2, V + 1, generator=g).mul_(2).to(dtype)
+    z = wide[:, 1:]  # from an element that is not 16-byte aligned
+    ids, t, up = torch.randint(0, V, (2, K), generator=g), torch.randn(2, K, generator=g), torch.rand(2, generator=g) + 1
+    want, q, p, slope, E = expected(z, ids, t, 1.0, cap)
+    dev = [wide.cuda()[:, 1:], ids.cuda(), t.cuda()]
+    loss, grad = distill_loss_grad(*dev, dloss=up.cuda(), softcap=cap)
+    tol = 2 * E[:, 0] + 2.0 ** -22 * want.abs()
+    assert ((loss.double().cpu() - want).abs() <= tol).all()
+    assert ((distill_loss(*dev, softcap=cap)[0].double().cpu() - want).abs() <= tol).all()
+    check_grad(grad, up, q, p, slope, E, 1.0, dtype)
