@@ -17,8 +17,9 @@
 // What it takes is bytes in flight and few instructions beside: a CTA is 128 threads, eight to an SM (one warp where
 // rows are many and short), and each thread copies its own 16-byte slots into shared memory some batches ahead (loads to
 // registers instead: a quarter more time; CTAs of 256 threads: 45 % more). Loss and gradient of 16,384 rows of 4,096
-// soft-capped fp32 logits with 32 entries: 102 us, 5.3 TB/s; 2,047 rows of 50,257 bf16 logits, the loss and then the
-// gradient from its lse: 130 us, 4.8 TB/s.
+// soft-capped fp32 logits with 32 entries: 98 to 104 us, 5.2 to 5.5 TB/s; the loss alone 54 us, 5.0 TB/s, since a row's copies
+// start and end with its CTA; 2,047 rows of 50,257 bf16 logits, the loss and then the gradient from its lse: 131 to 134
+// us, 4.6 TB/s.
 //
 // A row too long for one CTA, or one of a few rows, is spread over a cluster of up to 8 CTAs whose sums meet
 // through distributed shared memory, so no second launch or workspace is needed.
@@ -108,7 +109,7 @@ __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 ex2_pair(float2 x) { return make_float2(ex2_approx(x.x), ex2_approx(x.y)); }
 
 // tanh to about 2 ulp and its slope 1 - tanh^2 to about (4 |x| + 8) half ulp. Up to |x| = 1 from a polynomial x + x^3 Q(x^2): Q is a least-squares fit of degree 6 at Chebyshev
-// nodes, off by 6e-9 of tanh. Beyond, where 1 - e no longer cancels, from e = exp(-2 |x|): (1 - e) / (1 + e), and the slope
+// nodes, off by 1.3e-8 of tanh, 8.2e-8 as fp32 takes it. Beyond, where 1 - e no longer cancels, from e = exp(-2 |x|): (1 - e) / (1 + e), and the slope
 // as 4 e / (1 + e)^2, since 1 - tanh^2 would have lost all its digits at |x| = 9. Logits within the soft cap, nearly all
 // of a trained model's, so take no special function for their tanh.
 __device__ __forceinline__ float2 tanh_near(float2 x) {

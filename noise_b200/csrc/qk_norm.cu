@@ -17,9 +17,10 @@
 // different CTAs of one launch, so that the weight gradients need one accumulator set a thread.
 //
 // Measured: 8 + 8 heads of 64 in 16,384 tokens of a packed bf16 projection: 16.4 us, 4.1 TB/s. 12 + 4 heads of 96 in
-// 22,662 tokens with weights: forward 33 us, 4.2 TB/s, gradient 58 us, 3.6 TB/s, and 6 us for the weights' sums. Next to
-// HBM stand the instructions (120 a lane and row forward, 206 in the gradient; 60 % of the issue slots) and their
-// latency at 32 warps an SM. Eight values of either half a lane save instructions and cost registers: 97 against 60 us for
+// 22,662 tokens with weights: forward 37 us, 3.7 TB/s, gradient 63 us with the weights' sums, 3.3 TB/s; in fp32 50 and 79
+// us, 5.5 and 5.3 TB/s. Next to HBM stand the instructions (120 a lane and row forward, 206 in the gradient; 60 % of the
+// issue slots) and their latency at 32 warps an SM. A row takes a power of two of lanes, so that a quarter of them have no
+// columns at D = 96 and three eighths at 80: they take issue slots all the same. Eight values of either half a lane save instructions and cost registers: 97 against 60 us for
 // the gradient; copies through a ring in shared memory, 68 against 58; arithmetic without pairs, 24 instructions more,
 // the same time.
 #include <algorithm>

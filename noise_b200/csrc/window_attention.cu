@@ -21,17 +21,21 @@
 // tensor memory) two CTAs share an SM; at 128 (key tiles of 128) one CTA takes all 512 columns.
 //
 // Measured at B 8, T 2048, 8 heads of 64, window 1024, 4 sinks (bf16) and at T 16384, 16 heads on 4 key heads of
-// 128, window 4096, 64 sinks (fp16): 64 and 479 us, 405 and 1,020 TFLOP/s of visible pairs. The bound is the chain
-// S -> softmax -> P -> O of each tile and the products' rate: without any softmax work the same pipeline takes 53 and
-// 377 us, and the products alone 31 and 305 us at their measured rates (43 + N / 2 cycles for 16 values of the inner
-// dimension with both operands in shared memory, 11 + N / 2 with A in tensor memory). What other choices took, block
-// and long prompt, each against the kernel as it was then:
+// 128, window 4096, 64 sinks (fp16), in calls one after the other: 59 and 537 us, 435 and 907 TFLOP/s of visible pairs (the
+// long one slows the clock: 479 us in a few calls at 1,965 MHz). The bound is the chain S -> softmax -> P -> O of each tile
+// and the products' rate: without any softmax work the same pipeline takes 53 and 377 us (the latter at 1,965 MHz), and
+// the products alone 31 and 305 us at their measured rates (43 + N / 2 cycles for 16 values of the inner dimension with
+// both operands in shared memory, 11 + N / 2 with A in tensor memory). What other choices took, block and long prompt,
+// each against the kernel as it was then, in a few calls:
 //   a maximum of every tile: 153 against 102 us (both with the products issued from a one-lane branch)
 //   P in columns of its own beside S, one CTA an SM at 64: 84 and 551 against 76 and 504
 //   CTAs in launch order, not the heavy ones first: 76 and 504 against 64 and 479
 //   at 128, P handed over 64 keys at a time: 493 against 479; two warps a row: 494
 //   a quarter of the exponentials as polynomials on the fp32 units: 65 and 481 against 65 and 480
-// P is rounded to the input type, as the tensor core needs it; the row sum is of the unrounded values.
+// P is rounded to the input type, as the tensor core needs it; the row sum is of the unrounded values. The result is then
+// off by 2.1e-3 of its norm in bf16 and 2.5e-4 in fp16, where its own rounding makes 1.6e-3 and 2.0e-4. A second product
+// with what the rounding left takes the difference away (1.6e-3, 2.0e-4) and 76 and 698 us: eight softmax warps have to
+// split and store twice as much. Not kept for a part below the result's own rounding.
 //
 // A key tile that crosses the end of a padded sequence is loaded apart: the producer warp clears the value
 // rows behind the end before the products see them, since 0 times a NaN is not 0. Every wait is bounded.

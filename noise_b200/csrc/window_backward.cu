@@ -8,9 +8,10 @@
 //   window_stats:    Delta, and -lse in base 2, of every query row, in chunks of 64 rows the others load whole.
 //   window_backward: the keys' side, one CTA = 128 keys, streaming the 64-query tiles of every head of the group that
 //                    see them; then the queries' side, one CTA = 128 queries of one head, streaming the 64-key tiles.
-// S and dP are formed on both sides: 7 products a block of pairs instead of 5, but every gradient is summed in
-// one CTA's tensor memory in a fixed order. Adding dQ across key tiles with atomics would save the two products
-// and make the result depend on timing.
+// S and dP are formed on both sides, and dS goes into dQ and dK in two parts (below): 9 products a block of pairs where
+// the formulas have 5, and one of 16 columns for the addends. Every gradient is so summed in one CTA's tensor memory in a
+// fixed order. Adding dQ across key tiles with atomics would save S and dP a second time and make the result depend on
+// timing.
 //
 // The sides have one body. X0, X1 are the CTA's own 128-row tiles, Y0, Y1 the streamed 64-row tiles:
 //   S  = X0 Y0^T, dP = X1 Y1^T  (X in shared memory on the keys' side, in tensor memory, where its product is faster,
@@ -23,13 +24,14 @@
 // under S and -Delta under dP. Read from shared memory by every thread instead they took turns with the tensor core's
 // own reads: 240 us against 217.
 //
-// Measured (all launches) at B 8, T 2048, 8 heads of 64, window 1024, 4 sinks: 217 us, 298 TFLOP/s of the five products
+// Measured (all launches) at B 8, T 2048, 8 heads of 64, window 1024, 4 sinks: 220 us, 294 TFLOP/s of the five products
 // over the visible pairs; at 4 padded sequences of up to 1,999 tokens, 12 heads on 4 of 128, window 511, 16 sinks:
-// 110 us. What bounds it is each item's chain (S and dP, the warps' arithmetic, the gradients' products) at 64, the
+// 109 us. What bounds it is each item's chain (S and dP, the warps' arithmetic, the gradients' products) at 64, the
 // products' rate and a CTA's first and last item at 128. So two items are in flight per SM (two CTAs with one buffer of
 // S and dP each at 64, one CTA with two buffers at 128) and eight warps share an item, each with 32 rows and half of
 // the columns. One persistent CTA an SM with P and dS beside S and dP: 197 and 125 against 211 and 100 us.
-// P is rounded to bf16, as the tensor core needs. dS goes in as two bf16 numbers, its upper half (cut, which costs one
+// P is rounded to bf16, as the tensor core needs: dV is off by 2.3e-3 of its norm (1.7e-3 with the rest of P in a second
+// product, 235 against 220 us). dS goes in as two bf16 numbers, its upper half (cut, which costs one
 // permute a pair; rounded, 235 against 227 us) and the rest rounded, 16 bits in all, in the columns that dP lay in:
 // rounded to one, dQ and dK were off by 2.4e-3 of their norm where the rounding of the result alone makes 1.7e-3, and
 // the kernel took 20 us less. Sums are fp32.
