@@ -339,7 +339,7 @@ int noise_qk_norm_rope(const NoiseQkNorm* args, int backward, void* workspace, s
  * multiples of 16 bytes. Query row i of a sequence is at position p = offset + i (offset + Tq <= Tk) and
  * sees key j iff j <= p, and p - j <= window or j < sinks. lengths [B] (optional, on the device): tokens of
  * sequence b at positions >= lengths[b] are padding: their keys and values are never used, whatever they
- * hold, and their query rows give zeros (lse -inf).
+ * hold, and their query rows give zeros (lse -inf). So are keys and values behind the last query, for every sequence.
  * out [B, Tq, H, D] contiguous, 16-byte aligned; lse [B, H, Tq] fp32, the natural logarithm of each row's
  * sum of exp(scale q.k) over its visible keys. scale lies in [2^-100, 2^100]. Keys and values of tokens that are not
  * padding have to be finite: a hidden one still meets a probability of 0 in its tile. */

@@ -300,8 +300,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     first `sinks` keys; window None: every earlier key. q [B, Tq, H, D], k and v [B, Tk, Hk, D] of bf16 or fp16,
     H a multiple of Hk, D a multiple of 8 up to 128; query row i is at position offset + i (default offset
     Tk - Tq: the queries are the last ones). lengths: int32 [B] on the device; tokens of sequence b from lengths[b] on
-    are padding, whose keys and values are not used and whose query rows give zeros. A key or value of a
-    token that is not padding must be finite: it reaches the 128-query tiles of the queries that see it.
+    are padding, whose keys and values are not used and whose query rows give zeros. Keys and values behind the last
+    query (the free rows of a cache) are not used either. A key or value of another token must be finite: it reaches the
+    128-query tiles of the queries that see it.
     status: an int32 word that a device wait which ran out sets; without one the call waits for the
     GPU and checks its own. Returns (out [B, Tq, H, D], lse fp32 [B, H, Tq])."""
     name = 'window_attention'

@@ -16,9 +16,11 @@ struct WindowParams {
   int* status;
 };
 
-// Valid tokens of sequence b, within [0, Tk].
+// Tokens of sequence b that a query can see or be: those before its length and up to the last query. What lies behind, such
+// as the free rows of a cache, is padding whatever it holds.
 __device__ __forceinline__ int window_length(const WindowParams& p, int b) {
-  return p.lengths ? min(max(__ldg(p.lengths + b), 0), p.Tk) : p.Tk;
+  const int end = p.offset + p.Tq;
+  return p.lengths ? min(max(__ldg(p.lengths + b), 0), end) : end;
 }
 
 // Queries qlo .. qhi against keys klo .. khi: no pair visible, or every pair.

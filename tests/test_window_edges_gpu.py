@@ -56,3 +56,27 @@ def test_token_probabilities_have_two_parts(case):
             tol = tol + (n * v.double().abs().max() + 1) * 2.0 ** -25
         err = (out[b].double().cpu() - want[0, 0]).abs()
         assert (err <= tol[0, 0]).all(), (b, (err / tol[0, 0]).max())
+
+
+@pytest.mark.parametrize('D,H,Hk,Tq,Tk,offset,window,sinks,lengths', [
+    (64, 2, 1, 40, 300, 100, 64, 3, None), (128, 2, 2, 130, 512, 7, 200, 0, None), (64, 4, 2, 1, 200, 0, 5, 1, None),
+    (96, 3, 1, 257, 700, 130, 60, 140, (700, 300)), (128, 2, 1, 20, 150, 60, 20, 2, (70, 80)),
+])
+def test_rows_behind_the_last_query_hold_anything(D, H, Hk, Tq, Tk, offset, window, sinks, lengths):
+    """A prompt's part over a preallocated cache: the rows behind it are no key of any query, whatever they hold, and their
+    gradients are zero."""
+    from noise_b200.attention import window_attention, window_attention_backward
+    from test_window_gpu import check_backward, check_forward
+    g = torch.Generator().manual_seed(D + Tq)
+    B, bf = 2, torch.bfloat16
+    q, k, v, do = (randn(g, B, *s, D, dtype=bf) for s in ((Tq, H), (Tk, Hk), (Tk, Hk), (Tq, H)))
+    c = [x.cuda() for x in (q, k, v, do)]
+    c[1][:, offset + Tq:], c[2][:, offset + Tq:] = float('nan'), float('inf')
+    kw = dict(offset=offset)
+    if lengths:
+        kw['lengths'] = torch.tensor(lengths, dtype=torch.int32).cuda()
+    out, lse = window_attention(*c[:3], window, sinks, **kw)
+    check_forward(out, lse, q, k, v, window, sinks, lengths, offset, bf)
+    got = window_attention_backward(c[3], *c[:3], out, lse, window, sinks, **kw)
+    check_backward(got, do, q, k, v, window, sinks, lengths, offset)
+    assert (got[1][:, offset + Tq:] == 0).all() and (got[2][:, offset + Tq:] == 0).all()
